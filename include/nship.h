@@ -244,6 +244,85 @@ int nsh_op_muon_multi(int n, float* const* w, const float* const* g, const int64
  * place; codegen.cpp:3108-3119. */
 int nsh_op_adamw_step(float* w, const float* g, float* m, float* v, int64_t n, int64_t t, float lr);
 
+/* ---- experts chosen K a token, and Newton-Schulz updates --------------------
+ *
+ * No counterpart in the reference, whose mixture of experts is top-1 on its
+ * own router's product and whose Muon orthogonalises by Gram-Schmidt.  These
+ * calls enqueue on `stream` (a hipStream_t of the current device, where every
+ * buffer lies too; NULL = the null stream), return without waiting, allocate
+ * nothing and may be captured into a graph.  A call owns its workspace (and
+ * state) until it has run: calls that may overlap need one each.  Outputs do
+ * not overlap inputs or each other unless said so.  Workspaces and states are
+ * 16-byte aligned, of the size that their functions give (0: nothing needed,
+ * or sizes that the call refuses); the other buffers at any float.
+ *
+ * Sizes: E <= 1024 experts, K <= 64 choices, T K <= 2^24 slots. */
+
+/* Routing of T tokens to K of E experts each, from logits [T, E].
+ *   score 0: s = softmax of the row over its live experts, 1: s = 1 / (1 + e^-l)
+ *   c = s + bias (bias [E], NULL = 0: it steers the choice, not the weights)
+ *   top_groups < groups: the experts are `groups` runs of E / groups (at most
+ *   64 runs); a run counts by its largest c (group_best 1) or the sum of its
+ *   two largest (2); only the top_groups best runs are chosen from
+ * idx [T, K]: the experts of the K largest c, falling, equal ones by their
+ * index (as runs are); weight [T, K] = scale * s, over the sum of the token's
+ * K chosen s with renorm.  Scores are computed and compared in 64 bits.
+ * active [E] (bytes, NULL = all): 0 takes an expert out.  A logit of NaN or
+ * -inf takes the expert out for that token, a bias of NaN or -inf out of the
+ * choice.  Where fewer than K are left the rest of the row is idx -1, weight
+ * 0; a sum of 0 gives weights of 0. */
+int nsh_op_moe_route(const float* logits, const float* bias, const uint8_t* active, int32_t* idx, float* weight,
+                     int64_t T, int64_t E, int64_t K, int64_t groups, int64_t top_groups, int group_best, int score,
+                     int renorm, float scale, void* stream);
+
+/* The gradient of nsh_op_moe_route's weights: dlogits [T, E] from dweight
+ * [T, K], the choice (idx; the bias and the groups act through it alone) and
+ * the same logits, active, score, renorm and scale.  dweight of a slot whose
+ * idx is out of range or not live is not read; dlogits is 0 where an expert is
+ * not live. */
+int nsh_op_moe_route_grad(const float* dweight, const float* logits, const uint8_t* active, const int32_t* idx,
+                          float* dlogits, int64_t T, int64_t E, int64_t K, int score, int renorm, float scale,
+                          void* stream);
+
+/* The experts' products: y[t] = sum_k weight[t,k] act(x[t] W1[e]) W2[e] with e
+ * = idx[t,k], x and y [T, D], W1 [E, D, H], W2 [E, H, D]; act as nsh_op_gemm's.
+ * A slot whose idx is out of range adds nothing (its weight is not read); the
+ * same expert may stand in several slots of a token.  The sums' order depends
+ * on the sizes and idx alone: equal calls give equal bits.
+ * state (NULL for inference): keeps what the gradient needs. */
+size_t nsh_op_moe_experts_state(int64_t T, int64_t K, int64_t D, int64_t H, int64_t E);
+size_t nsh_op_moe_experts_workspace(int64_t T, int64_t K, int64_t D, int64_t H, int64_t E, int grad);
+int nsh_op_moe_experts(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2,
+                       float* y, int64_t T, int64_t K, int64_t D, int64_t H, int64_t E, int act, void* state,
+                       void* workspace, void* stream);
+
+/* Its gradients from dy [T, D], the same x, weight, W1, W2, act and the
+ * forward's state: dx [T, D], dweight [T, K] (0 for slots without an expert),
+ * dW1 [E, D, H], dW2 [E, H, D] (0 for experts without tokens), each written
+ * whole; any may be NULL.  workspace: nsh_op_moe_experts_workspace(..., 1),
+ * which serves the forward too.  T = 0 takes no state and no workspace. */
+int nsh_op_moe_experts_grad(const float* dy, const float* x, const float* weight, const float* W1, const float* W2,
+                            const void* state, float* dx, float* dweight, float* dW1, float* dW2, int64_t T,
+                            int64_t K, int64_t D, int64_t H, int64_t E, int act, void* workspace, void* stream);
+
+/* Orthogonalisation of n matrices [r, c] by Newton-Schulz products:
+ *   X = G / (|G|_F + 1e-7); `steps` times (5 as a rule): A = X X^T,
+ *   X = 3.4445 X + (-4.7750 A + 2.0315 A A) X   (X^T X where r > c)
+ * g, q [n, r, c]; q may be g.  A matrix with an infinity or NaN comes out as
+ * NaN, a zero one as zeros; the others of the batch are not touched by it.
+ * n <= 65535, min(r, c) <= 32768, max(r, c) <= 2^22. */
+size_t nsh_op_newton_schulz_workspace(int64_t n, int64_t r, int64_t c);
+int nsh_op_newton_schulz(const float* g, float* q, int64_t n, int64_t r, int64_t c, int steps, void* workspace,
+                         void* stream);
+
+/* The Muon step of n matrices [r, c] on such an update:
+ *   m = mu m + g;  u = nesterov ? g + mu m : m    (m NULL: u = g)
+ *   w -= lr sqrt(min(r, c)) NS(u) + 0.01 lr w
+ * i.e. nsh_op_muon_step's rule.  w and m are updated in place.  workspace:
+ * nsh_op_newton_schulz_workspace. */
+int nsh_op_muon_ns_step(float* w, const float* g, float* m, int64_t n, int64_t r, int64_t c, float lr, float mu,
+                        int nesterov, int steps, void* workspace, void* stream);
+
 /* Attainable peaks of the running GPU (no reference counterpart: the
  * reference has no timing).  nsh_bench_mfma_peak: register-only fp32 MFMA
  * loop, blocks x 256 threads, iters x 4 MFMA 32x32x2 per wave (4096 FLOP

@@ -254,4 +254,60 @@ int launch_moe_backward(const float* x, const float* dout, const float* Wg, cons
                         float* dWe1, float* dWe2, int64_t M, int64_t D, int64_t H, int64_t E, hipStream_t s,
                         int phases = kMoeBwdAll);
 
+// moe_topk.hip -----------------------------------------------------------------
+// Most experts that the routing and the layer with K experts a token take, and
+// most choices (one lane of a wave each) and groups.
+constexpr int kMoeMaxExperts = 1024, kMoeMaxChoices = 64;
+// Most tokens, and most slots (tokens times choices): grids of a wave a slot.
+constexpr int64_t kMoeMaxSlots = 1 << 24;
+struct RouteArgs {
+  const float* logits;    // [T, E]
+  const float* bias;      // [E] or null
+  const uint8_t* active;  // [E] or null
+  int32_t* idx;           // [T, K]
+  float* weight;          // [T, K]
+  int64_t T;
+  int E, K, groups, top_groups, group_best;
+  int score;   // 0 softmax, 1 sigmoid
+  int renorm;  // weights over their sum
+  float scale;
+};
+struct RouteGradArgs {
+  const float* dweight;   // [T, K]
+  const float* logits;
+  const uint8_t* active;
+  const int32_t* idx;
+  float* dlogits;         // [T, E]
+  int64_t T;
+  int E, K, score, renorm;
+  float scale;
+};
+int launch_route(const RouteArgs& a, hipStream_t s);
+int launch_route_grad(const RouteGradArgs& a, hipStream_t s);
+
+struct MoeShape {
+  int64_t T, K, D, H, E;
+};
+size_t experts_state_bytes(const MoeShape& m);
+size_t experts_workspace_bytes(const MoeShape& m, bool grad);
+int launch_experts(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2, float* y,
+                   const MoeShape& m, int act, void* state, void* workspace, hipStream_t s);
+int launch_experts_grad(const float* dy, const float* x, const float* weight, const float* W1, const float* W2,
+                        const void* state, float* dx, float* dweight, float* dW1, float* dW2, const MoeShape& m,
+                        int act, void* workspace, hipStream_t s);
+
+// newton.hip -------------------------------------------------------------------
+// Orthogonalisation of n matrices [r, c] by `steps` Newton-Schulz products.
+// step null: q = the result of g.  Else the Muon update: m = mu m + g (m not
+// null), u = nesterov ? g + mu m : m, w = w - le NS(u) - decay w.
+struct MuonNs {
+  float* w;
+  float* m;
+  float mu, le, decay;
+  int nesterov;
+};
+size_t newton_schulz_bytes(int64_t n, int64_t r, int64_t c);
+int launch_newton_schulz(const float* g, float* q, const MuonNs* step, int64_t n, int64_t r, int64_t c, int steps,
+                         void* workspace, hipStream_t s);
+
 }  // namespace nship

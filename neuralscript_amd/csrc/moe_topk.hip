@@ -1,0 +1,545 @@
+// Mixture of experts with K experts a token: routing from given logits and its
+// gradient, and the experts' products forward and backward.
+//
+//   routing   s = softmax(l) or 1 / (1 + e^-l) over the live experts, c = s + bias;
+//             the best groups stay, the K largest c of them are chosen, and
+//             weight_k = scale s_k (/ sum_j s_j)
+//   layer     y_t = sum_k weight_tk act(x_t W1[e]) W2[e],  e = idx_tk
+//
+// A (token, choice) pair t K + k is a slot.  The layer sorts the slots by
+// expert (stable, so every sum has one order) and runs grouped products over
+// the sorted rows; the slots of a token meet in a pass of their own, in the
+// order of k.
+#include <algorithm>
+
+#include "common.h"
+#include "kernels.h"
+
+namespace nship {
+namespace {
+
+constexpr double kNone = -__builtin_inf();
+
+__device__ __forceinline__ double shfl_xor_f64(double v, int o) { return __shfl_xor(v, o, kWave); }
+
+// The logit of expert e, -inf where the expert is not live.  Written without a
+// branch on the lane: as `if (dead) x = -inf` hipcc 7.2 drops the assignment
+// of every register but the first.
+__device__ __forceinline__ float live_logit(const float* __restrict__ l, int e, int E,
+                                            const uint8_t* __restrict__ active) {
+  const bool in = e >= 0 && e < E;
+  const int at = in ? e : 0;
+  const float x = l[at];
+  const int on = active ? active[at] : 1;  // (uniform)
+  return (int)in & (int)(on != 0) & (int)(x > -__builtin_inff()) ? x : -__builtin_inff();  // (NaN > -inf is false)
+}
+
+// The larger value over the wave, the lower index on a tie.
+__device__ __forceinline__ void wave_best(double& v, int& i) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const double w = shfl_xor_f64(v, o);
+    const int j = __shfl_xor(i, o, kWave);
+    const bool take = w > v || (w == v && j < i);
+    v = take ? w : v;
+    i = take ? j : i;
+  }
+}
+
+// One wave per token, expert v 64 + lane in register v.  The scores and what
+// they are compared by are held in 64 bits: a choice is an integer, and two
+// values 2^-24 apart, which 32 bits may order either way, turn up in every few
+// thousand tokens.
+template <int V>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
+  __shared__ double by_expert[4][64 * V];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t tok = (int64_t)blockIdx.x * 4 + w;
+  if (tok >= a.T) return;  // (uniform per wave; no barrier below)
+  const float* __restrict__ l = a.logits + tok * a.E;
+  double s[V], c[V];
+  float x[V], mx = -__builtin_inff();
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    x[v] = live_logit(l, v * 64 + lane, a.E, a.active);
+    mx = fmaxf(mx, x[v]);
+  }
+  mx = wave_max(mx);
+  if (a.score == 0) {
+    double sum = 0.;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const bool live = x[v] > -__builtin_inff();
+      s[v] = !live ? 0. : x[v] == mx ? 1. : exp((double)x[v] - (double)mx);  // (a logit of +inf: 1)
+      sum += s[v];
+    }
+    sum = wave_sum(sum);
+#pragma unroll
+    for (int v = 0; v < V; v++) s[v] = sum > 0. ? s[v] / sum : 0.;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; v++) s[v] = x[v] > -__builtin_inff() ? 1. / (1. + exp(-(double)x[v])) : 0.;
+  }
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const int e = v * 64 + lane;
+    const double b = s[v] + (a.bias ? (double)a.bias[e < a.E ? e : 0] : 0.);
+    c[v] = (int)(x[v] > -__builtin_inff()) & (int)(b > kNone) ? b : kNone;  // (a NaN bias: never chosen)
+  }
+  if (a.groups > 1) {
+    const int per = a.E / a.groups;
+    double* __restrict__ t = by_expert[w];
+#pragma unroll
+    for (int v = 0; v < V; v++) t[v * 64 + lane] = c[v];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    double one = kNone, two = kNone;
+    if (lane < a.groups)
+      for (int j = 0; j < per; j++) {
+        const double b = t[lane * per + j];
+        two = b > one ? one : b > two ? b : two;
+        one = b > one ? b : one;
+      }
+    if (a.group_best == 2 && two > kNone) one += two;
+    uint64_t keep = 0;
+    for (int g = 0; g < a.top_groups; g++) {
+      double v = one;
+      int i = lane;
+      wave_best(v, i);
+      if (!(v > kNone)) break;
+      keep |= 1ull << i;
+      if (lane == i) one = kNone;
+    }
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const int e = v * 64 + lane;
+      c[v] = (keep >> (min(e, a.E - 1) / per)) & 1 ? c[v] : kNone;
+    }
+  }
+  int mine = -1;
+  double ms = 0.;
+  for (int k = 0; k < a.K; k++) {
+    double v = c[0], sv = s[0];
+    int i = lane;
+#pragma unroll
+    for (int u = 1; u < V; u++) {
+      const bool more = c[u] > v;
+      v = more ? c[u] : v;
+      sv = more ? s[u] : sv;
+      i = more ? u * 64 + lane : i;
+    }
+    const int own = i;
+    wave_best(v, i);
+    if (!(v > kNone)) break;
+    sv = __shfl(sv, i & 63, kWave);
+    if (lane == k) {
+      mine = i;
+      ms = sv;
+    }
+#pragma unroll
+    for (int u = 0; u < V; u++) c[u] = own == i && u == i >> 6 ? kNone : c[u];
+  }
+  double by = 1.;
+  if (a.renorm) by = wave_sum(ms);
+  if (lane < a.K) {
+    a.idx[tok * a.K + lane] = mine;
+    a.weight[tok * a.K + lane] = by > 0. ? (float)((double)a.scale * ms / by) : 0.f;
+  }
+}
+
+// One wave per token; lane k holds choice k.
+template <int V>
+__global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t tok = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (tok >= a.T) return;
+  const float* __restrict__ l = a.logits + tok * a.E;
+  float x[V], s[V], mx = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    x[v] = live_logit(l, v * 64 + lane, a.E, a.active);
+    mx = fmaxf(mx, x[v]);
+  }
+  mx = wave_max(mx);
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const bool live = x[v] > -__builtin_inff();
+    s[v] = !live ? 0.f : a.score ? 1.f / (1.f + expf(-x[v])) : x[v] == mx ? 1.f : expf(x[v] - mx);
+    sum += s[v];
+  }
+  const float by = a.score ? 1.f : wave_sum(sum);
+  // this lane's choice, its score and the derivative by that score
+  int mine = -1;
+  float u = 0.f, sk = 0.f;
+  float xm = -__builtin_inff();
+  if (lane < a.K) {
+    mine = a.idx[tok * a.K + lane];
+    xm = live_logit(l, mine, a.E, a.active);
+  }
+  mine = xm > -__builtin_inff() ? mine : -1;
+  if (mine >= 0) {
+    sk = a.score ? 1.f / (1.f + expf(-xm)) : (xm == mx ? 1.f : expf(xm - mx)) / by;
+    u = a.dweight[tok * a.K + lane] * a.scale;
+  }
+  if (a.renorm) {
+    const float total = wave_sum(sk), dot = wave_sum(u * sk);
+    u = mine >= 0 && total > 0.f ? (u - dot / total) / total : 0.f;
+  }
+  const float dot = a.score ? 0.f : wave_sum(u * sk);
+  float ds[V];
+#pragma unroll
+  for (int v = 0; v < V; v++) ds[v] = 0.f;
+  for (int k = 0; k < a.K; k++) {
+    const int e = __builtin_amdgcn_readlane(mine, k);
+    const float d = read_lane(u, k);
+#pragma unroll
+    for (int v = 0; v < V; v++) ds[v] += e == v * 64 + lane ? d : 0.f;
+  }
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const int e = v * 64 + lane;
+    if (e >= a.E) continue;
+    const float p = by > 0.f ? s[v] / by : 0.f;  // (0: no expert is live)
+    a.dlogits[tok * a.E + e] = a.score ? p * (1.f - p) * ds[v] : p * (ds[v] - dot);
+  }
+}
+
+// ---- slots sorted by expert -------------------------------------------------------
+
+constexpr int kSortBlock = 1024;  // slots a workgroup
+
+// A wave's lanes that hold the same expert (e in [0, E), E <= 1024; -1: none).
+__device__ __forceinline__ uint64_t same_expert(int e) {
+  uint64_t m = __ballot(e >= 0);
+#pragma unroll
+  for (int b = 0; b < 10; b++) {
+    const uint64_t set = __ballot((e >> b) & 1);
+    m &= (e >> b) & 1 ? set : ~set;
+  }
+  return e >= 0 ? m : 0;
+}
+__device__ __forceinline__ int slot_expert(const int32_t* __restrict__ idx, int64_t i, int64_t N, int E) {
+  if (i >= N) return -1;
+  const int e = idx[i];
+  return e >= 0 && e < E ? e : -1;
+}
+
+// count[block][e]: the block's slots of each expert.
+__global__ __launch_bounds__(kSortBlock) void slots_count_kernel(const int32_t* __restrict__ idx, int64_t N, int E,
+                                                                 int* __restrict__ count) {
+  __shared__ int c[kMoeMaxExperts];
+  for (int e = threadIdx.x; e < E; e += kSortBlock) c[e] = 0;
+  __syncthreads();
+  const int e = slot_expert(idx, (int64_t)blockIdx.x * kSortBlock + threadIdx.x, N, E);
+  const uint64_t m = same_expert(e);
+  if (e >= 0 && (threadIdx.x & 63) == __builtin_ctzll(m)) atomicAdd(&c[e], __builtin_popcountll(m));
+  __syncthreads();
+  for (int i = threadIdx.x; i < E; i += kSortBlock) count[(int64_t)blockIdx.x * E + i] = c[i];
+}
+
+// Each expert's segment, the blocks' offsets in it (in place of their counts)
+// and the (expert, tile of 128 rows) list.  One workgroup, thread e an expert.
+__global__ __launch_bounds__(kMoeMaxExperts) void slots_scan_kernel(int* __restrict__ count, int nblk, int E,
+                                                                    int* __restrict__ seg, int* __restrict__ tiles,
+                                                                    int* __restrict__ ntiles) {
+  __shared__ int n[kMoeMaxExperts], t[kMoeMaxExperts];
+  const int e = threadIdx.x;
+  int total = 0;
+  if (e < E)
+    for (int b = 0; b < nblk; b++) total += count[(int64_t)b * E + e];
+  n[e] = total;
+  t[e] = (total + 127) / 128;
+  for (int o = 1; o < kMoeMaxExperts; o <<= 1) {
+    __syncthreads();
+    const int pn = e >= o ? n[e - o] : 0, pt = e >= o ? t[e - o] : 0;
+    __syncthreads();
+    n[e] += pn;
+    t[e] += pt;
+  }
+  __syncthreads();
+  if (e >= E) return;
+  const int nt = (total + 127) / 128;
+  int at = n[e] - total;
+  seg[e] = at;
+  if (e == E - 1) {
+    seg[E] = n[e];
+    *ntiles = t[e];
+  }
+  for (int b = 0; b < nblk; b++) {
+    const int c = count[(int64_t)b * E + e];
+    count[(int64_t)b * E + e] = at;
+    at += c;
+  }
+  for (int i = 0; i < nt; i++) {
+    tiles[2 * (t[e] - nt + i)] = e;
+    tiles[2 * (t[e] - nt + i) + 1] = i;
+  }
+}
+
+// perm[position] = slot, tok[position] = its token (stable), expert[slot].
+__global__ __launch_bounds__(kSortBlock) void slots_place_kernel(const int32_t* __restrict__ idx, int64_t N, int E,
+                                                                 int K, const int* __restrict__ offset,
+                                                                 int* __restrict__ perm, int* __restrict__ tok,
+                                                                 int* __restrict__ expert) {
+  __shared__ int c[16][kMoeMaxExperts];  // slots of each expert in the waves before
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  for (int i = threadIdx.x; i < 16 * E; i += kSortBlock) c[i / E][i % E] = 0;
+  __syncthreads();
+  const int64_t slot = (int64_t)blockIdx.x * kSortBlock + threadIdx.x;
+  const int e = slot_expert(idx, slot, N, E);
+  if (slot < N) expert[slot] = e;
+  const uint64_t m = same_expert(e);
+  const int rank = __builtin_popcountll(m & ((1ull << lane) - 1));
+  if (e >= 0 && rank == 0) c[w][e] = __builtin_popcountll(m);
+  __syncthreads();
+  if (e < 0) return;
+  int at = offset[(int64_t)blockIdx.x * E + e] + rank;
+  for (int u = 0; u < w; u++) at += c[u][e];
+  perm[at] = (int)slot;
+  tok[at] = (int)(slot / K);
+}
+
+// ---- rows ---------------------------------------------------------------------------
+
+// h = act(u) over the rows [0, *nrows) of H
+__global__ __launch_bounds__(256) void act_rows_kernel(const float* __restrict__ u, float* __restrict__ h,
+                                                       const int* __restrict__ nrows, int64_t H, int act) {
+  const int64_t n = (int64_t)*nrows * H;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    h[i] = act_apply(u[i], act);
+}
+
+// y[t] = sum over the token's slots, in order, of o[slot]; slots without an
+// expert add nothing (their rows of o are not written).
+template <int W>
+__global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ o, const int* __restrict__ expert,
+                                                      float* __restrict__ y, int64_t T, int K, int64_t DW) {
+  const int64_t n = T * DW;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = i / DW, c = i - t * DW;
+    float v[W];
+#pragma unroll
+    for (int j = 0; j < W; j++) v[j] = 0.f;
+    for (int k = 0; k < K; k++) {
+      if (expert[t * K + k] < 0) continue;
+      const float* p = o + ((t * K + k) * DW + c) * W;
+#pragma unroll
+      for (int j = 0; j < W; j++) v[j] += p[j];
+    }
+#pragma unroll
+    for (int j = 0; j < W; j++) y[i * W + j] = v[j];
+  }
+}
+
+// act'(u).  SiLU's is sigma (1 + u (1 - sigma)); the networks' own layers take
+// the reference's spelling (act_deriv), which is another function.
+__device__ __forceinline__ float act_slope(float u, int act) {
+  if (act != kActSilu) return act_deriv(u, act);
+  const float s = 1.f / (1.f + expf(-u));
+  return s + u * s * (1.f - s);
+}
+
+// One wave per sorted row: dweight = act(u) . dh, du = weight act'(u) dh (in
+// place of dh), hw = weight act(u).
+__global__ __launch_bounds__(256) void bwd_rows_kernel(const float* __restrict__ pre, float* __restrict__ dh,
+                                                       float* __restrict__ hw, const float* __restrict__ weight,
+                                                       float* __restrict__ dweight, const int* __restrict__ perm,
+                                                       const int* __restrict__ nrows, int H, int act) {
+  const int lane = threadIdx.x & 63;
+  const int64_t pos = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (pos >= *nrows) return;
+  const int slot = perm[pos];
+  const float w = weight[slot];
+  float dot = 0.f;
+  for (int a = lane; a < H; a += 64) {
+    const float u = pre[pos * H + a], d = dh[pos * H + a], h = act_apply(u, act);
+    dot += h * d;
+    dh[pos * H + a] = w * d * act_slope(u, act);
+    hw[pos * H + a] = w * h;
+  }
+  dot = wave_sum(dot);
+  if (dweight && lane == 0) dweight[slot] = dot;
+}
+
+// a2[pos] = a[tok[pos]], b2 alike
+__global__ __launch_bounds__(256) void gather_kernel(const float* __restrict__ a, const float* __restrict__ b,
+                                                     const int* __restrict__ tok, const int* __restrict__ nrows,
+                                                     float* __restrict__ a2, float* __restrict__ b2, int64_t D) {
+  const int64_t n = (int64_t)*nrows * D;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / D, src = (int64_t)tok[r] * D + (i - r * D);
+    a2[i] = a[src];
+    b2[i] = b[src];
+  }
+}
+
+struct Tables {
+  int *seg, *perm, *tok, *expert, *tiles, *ntiles;
+};
+constexpr int64_t round64(int64_t n) { return (n + 63) / 64 * 64; }
+int64_t tables_ints(int64_t N, int64_t E) {
+  return round64(E + 1) + 3 * round64(N) + round64(2 * (ceil_div(N, 128) + E)) + 64;
+}
+Tables tables_at(int* p, int64_t N, int64_t E) {
+  Tables t;
+  t.seg = p;
+  t.perm = t.seg + round64(E + 1);
+  t.tok = t.perm + round64(N);
+  t.expert = t.tok + round64(N);
+  t.tiles = t.expert + round64(N);
+  t.ntiles = t.tiles + round64(2 * (ceil_div(N, 128) + E));
+  return t;
+}
+int64_t count_ints(int64_t N, int64_t E) { return round64(ceil_div(N, kSortBlock) * E); }
+
+int sort_slots(const int32_t* idx, const Tables& t, int* count, int64_t N, int K, int E, hipStream_t s) {
+  const int nblk = (int)ceil_div(N, kSortBlock);
+  hipLaunchKernelGGL(slots_count_kernel, dim3(nblk), dim3(kSortBlock), 0, s, idx, N, E, count);
+  NSH_LAUNCHED();
+  hipLaunchKernelGGL(slots_scan_kernel, dim3(1), dim3(kMoeMaxExperts), 0, s, count, nblk, E, t.seg, t.tiles, t.ntiles);
+  NSH_LAUNCHED();
+  hipLaunchKernelGGL(slots_place_kernel, dim3(nblk), dim3(kSortBlock), 0, s, idx, N, E, K, count, t.perm, t.tok,
+                     t.expert);
+  NSH_LAUNCHED();
+  return 0;
+}
+
+unsigned stream_blocks(int64_t n) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(n, 256), 8192)); }
+
+int launch_combine(const float* o, const int* expert, float* y, const MoeShape& m, hipStream_t s) {
+  if (m.D % 4 == 0 && ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(y)) & 15) == 0)
+    hipLaunchKernelGGL(combine_kernel<4>, dim3(stream_blocks(m.T * m.D / 4)), dim3(256), 0, s, o, expert, y, m.T,
+                       (int)m.K, m.D / 4);
+  else
+    hipLaunchKernelGGL(combine_kernel<1>, dim3(stream_blocks(m.T * m.D)), dim3(256), 0, s, o, expert, y, m.T, (int)m.K,
+                       m.D);
+  NSH_LAUNCHED();
+  return 0;
+}
+
+GemmArgs grouped(const Tables& t, int64_t rows, int64_t N, int64_t K, const float* A, const float* B, float* C,
+                 const MoeShape& m, bool tB) {
+  GemmArgs g;
+  g.A = A; g.B = B; g.C = C;
+  g.M = (int)rows; g.N = (int)N; g.K = (int)K;
+  g.lda = K; g.ldb = tB ? K : N; g.ldc = N;
+  g.groups = (int)m.E; g.seg = t.seg; g.tiles = t.tiles; g.ntiles = t.ntiles; g.sBg = N * K;
+  return g;
+}
+
+}  // namespace
+
+int launch_route(const RouteArgs& a, hipStream_t s) {
+  if (a.T <= 0) return 0;
+  const dim3 g((unsigned)ceil_div(a.T, 4));
+  if (a.E <= 64) hipLaunchKernelGGL(route_kernel<1>, g, dim3(256), 0, s, a);
+  else if (a.E <= 128) hipLaunchKernelGGL(route_kernel<2>, g, dim3(256), 0, s, a);
+  else if (a.E <= 256) hipLaunchKernelGGL(route_kernel<4>, g, dim3(256), 0, s, a);
+  else if (a.E <= 512) hipLaunchKernelGGL(route_kernel<8>, g, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(route_kernel<16>, g, dim3(256), 0, s, a);
+  NSH_LAUNCHED();
+  return 0;
+}
+
+int launch_route_grad(const RouteGradArgs& a, hipStream_t s) {
+  if (a.T <= 0) return 0;
+  const dim3 g((unsigned)ceil_div(a.T, 4));
+  if (a.E <= 64) hipLaunchKernelGGL(route_grad_kernel<1>, g, dim3(256), 0, s, a);
+  else if (a.E <= 128) hipLaunchKernelGGL(route_grad_kernel<2>, g, dim3(256), 0, s, a);
+  else if (a.E <= 256) hipLaunchKernelGGL(route_grad_kernel<4>, g, dim3(256), 0, s, a);
+  else if (a.E <= 512) hipLaunchKernelGGL(route_grad_kernel<8>, g, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(route_grad_kernel<16>, g, dim3(256), 0, s, a);
+  NSH_LAUNCHED();
+  return 0;
+}
+
+// state: the sorted slots' tables, then the pre-activations [T K, H]
+size_t experts_state_bytes(const MoeShape& m) {
+  const int64_t N = m.T * m.K;
+  return 4 * (size_t)(tables_ints(N, m.E) + N * m.H);
+}
+// workspace: the sort's counts, the tables (no state), then of the forward
+// hidden [N, H] and slots [N, D]; of the backward dh, hw [N, H], x and dy
+// sorted and the slots [N, D]
+size_t experts_workspace_bytes(const MoeShape& m, bool grad) {
+  const int64_t N = m.T * m.K;
+  const int64_t fwd = count_ints(N, m.E) + tables_ints(N, m.E) + round64(N * m.H) + N * m.D;
+  const int64_t bwd = 2 * round64(N * m.H) + 3 * round64(N * m.D);
+  return 4 * (size_t)std::max(fwd, grad ? bwd : 0);
+}
+
+int launch_experts(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2, float* y,
+                   const MoeShape& m, int act, void* state, void* workspace, hipStream_t s) {
+  const int64_t N = m.T * m.K;
+  if (m.T <= 0 || m.D <= 0) return 0;
+  int* wi = static_cast<int*>(workspace);
+  int* count = wi;
+  wi += count_ints(N, m.E);
+  int* ti = state ? static_cast<int*>(state) : wi;
+  if (!state) wi += tables_ints(N, m.E);
+  float* hidden = reinterpret_cast<float*>(wi);
+  float* slots = hidden + round64(N * m.H);
+  const Tables t = tables_at(ti, N, m.E);
+  float* pre = hidden;
+  if (state) pre = reinterpret_cast<float*>(ti + tables_ints(N, m.E));
+  if (sort_slots(idx, t, count, N, (int)m.K, (int)m.E, s) != 0) return -1;
+  GemmArgs g = grouped(t, N, m.H, m.D, x, W1, pre, m, false);
+  g.a_rows = t.tok;
+  if (launch_gemm_ex(g, false, false, 1, s) != 0) return -1;
+  hipLaunchKernelGGL(act_rows_kernel, dim3(stream_blocks(N * m.H)), dim3(256), 0, s, pre, hidden, t.seg + m.E, m.H, act);
+  NSH_LAUNCHED();
+  GemmArgs g2 = grouped(t, N, m.D, m.H, hidden, W2, slots, m, false);
+  g2.c_rows = t.perm;
+  g2.row_scale = weight;
+  if (launch_gemm_ex(g2, false, false, 1, s) != 0) return -1;
+  return launch_combine(slots, t.expert, y, m, s);
+}
+
+int launch_experts_grad(const float* dy, const float* x, const float* weight, const float* W1, const float* W2,
+                        const void* state, float* dx, float* dweight, float* dW1, float* dW2, const MoeShape& m,
+                        int act, void* workspace, hipStream_t s) {
+  const int64_t N = m.T * m.K;
+  if (N <= 0 || m.D <= 0) {
+    if (dW1 && launch_fill(dW1, m.E * m.D * m.H, 0.f, s) != 0) return -1;
+    if (dW2 && launch_fill(dW2, m.E * m.D * m.H, 0.f, s) != 0) return -1;
+    return dweight ? launch_fill(dweight, N, 0.f, s) : 0;
+  }
+  int* ti = const_cast<int*>(static_cast<const int*>(state));
+  const Tables t = tables_at(ti, N, m.E);
+  const float* pre = reinterpret_cast<const float*>(ti + tables_ints(N, m.E));
+  float* dh = static_cast<float*>(workspace);
+  float* hw = dh + round64(N * m.H);
+  float* xs = hw + round64(N * m.H);
+  float* dys = xs + round64(N * m.D);
+  float* slots = dys + round64(N * m.D);
+  const int* nrows = t.seg + m.E;
+  GemmArgs g = grouped(t, N, m.H, m.D, dy, W2, dh, m, true);
+  g.a_rows = t.tok;
+  if (launch_gemm_ex(g, false, true, 1, s) != 0) return -1;
+  if (dweight && launch_fill(dweight, N, 0.f, s) != 0) return -1;
+  hipLaunchKernelGGL(bwd_rows_kernel, dim3((unsigned)ceil_div(N, 4)), dim3(256), 0, s, pre, dh, hw, weight, dweight,
+                     t.perm, nrows, (int)m.H, act);
+  NSH_LAUNCHED();
+  if (dx) {
+    GemmArgs h = grouped(t, N, m.D, m.H, dh, W1, slots, m, true);
+    h.c_rows = t.perm;
+    if (launch_gemm_ex(h, false, true, 1, s) != 0) return -1;
+    if (launch_combine(slots, t.expert, dx, m, s) != 0) return -1;
+  }
+  if (!dW1 && !dW2) return 0;
+  hipLaunchKernelGGL(gather_kernel, dim3(stream_blocks(N * m.D)), dim3(256), 0, s, x, dy, t.tok, nrows, xs, dys, m.D);
+  NSH_LAUNCHED();
+  auto weight_grad = [&](const float* A, const float* B, float* C, int64_t R, int64_t Cc) {
+    GemmArgs k;
+    k.A = A; k.B = B; k.C = C;
+    k.M = (int)R; k.N = (int)Cc; k.K = (int)N;
+    k.lda = R; k.ldb = Cc; k.ldc = Cc;
+    k.sC = R * Cc;
+    k.kseg = t.seg;
+    return launch_gemm_ex(k, true, false, (int)m.E, s);
+  };
+  if (dW1 && weight_grad(xs, dh, dW1, m.D, m.H) != 0) return -1;
+  if (dW2 && weight_grad(hw, dys, dW2, m.H, m.D) != 0) return -1;
+  return 0;
+}
+
+}  // namespace nship

@@ -2116,4 +2116,121 @@ int nsh_op_attention_bwd(const float* Q, const float* K, const float* V, const f
   return 0;
 }
 
+// ---- experts chosen K a token, Newton-Schulz updates: on the caller's stream ----
+
+// Whether work on `stream` runs on the current device, as the buffers must.
+static bool stream_here(hipStream_t stream, const char* what) {
+  if (!stream) return true;
+  hipDevice_t of = 0;
+  int cur = 0;
+  if (hipStreamGetDevice(stream, &of) != hipSuccess || hipGetDevice(&cur) != hipSuccess || (int)of != cur) {
+    (void)hipGetLastError();
+    set_error(std::string(what) + ": the stream is not one of the current device");
+    return false;
+  }
+  return true;
+}
+
+int nsh_op_moe_route(const float* logits, const float* bias, const uint8_t* active, int32_t* idx, float* weight,
+                     int64_t T, int64_t E, int64_t K, int64_t groups, int64_t top_groups, int group_best, int score,
+                     int renorm, float scale, void* stream) {
+  NSH_OP_REQUIRE(T >= 0 && T <= kMoeMaxSlots && E >= 1 && E <= kMoeMaxExperts && K >= 1 && K <= kMoeMaxChoices &&
+                     K <= E && groups >= 1 && groups <= 64 && E % groups == 0 && top_groups >= 1 &&
+                     top_groups <= groups && (group_best == 1 || group_best == 2) && (score == 0 || score == 1) &&
+                     (T == 0 || (logits && idx && weight)),
+                 "moe_route");
+  if (!stream_here((hipStream_t)stream, "moe_route")) return -1;
+  RouteArgs a;
+  a.logits = logits; a.bias = bias; a.active = active; a.idx = idx; a.weight = weight;
+  a.T = T; a.E = (int)E; a.K = (int)K;
+  a.groups = top_groups < groups ? (int)groups : 1;  // (all groups stay: no groups)
+  a.top_groups = (int)top_groups; a.group_best = group_best;
+  a.score = score; a.renorm = renorm != 0; a.scale = scale;
+  return launch_route(a, (hipStream_t)stream);
+}
+
+int nsh_op_moe_route_grad(const float* dweight, const float* logits, const uint8_t* active, const int32_t* idx,
+                          float* dlogits, int64_t T, int64_t E, int64_t K, int score, int renorm, float scale,
+                          void* stream) {
+  NSH_OP_REQUIRE(T >= 0 && T <= kMoeMaxSlots && E >= 1 && E <= kMoeMaxExperts && K >= 1 && K <= kMoeMaxChoices &&
+                     (score == 0 || score == 1) && (T == 0 || (dweight && logits && idx && dlogits)),
+                 "moe_route_grad");
+  if (!stream_here((hipStream_t)stream, "moe_route_grad")) return -1;
+  RouteGradArgs a;
+  a.dweight = dweight; a.logits = logits; a.active = active; a.idx = idx; a.dlogits = dlogits;
+  a.T = T; a.E = (int)E; a.K = (int)K;
+  a.score = score; a.renorm = renorm != 0; a.scale = scale;
+  return launch_route_grad(a, (hipStream_t)stream);
+}
+
+// Sizes that the layer's kernels and grids can index (T K slots of D or H).
+static bool moe_shape_ok(int64_t T, int64_t K, int64_t D, int64_t H, int64_t E) {
+  if (T < 0 || T > kMoeMaxSlots || K < 1 || K > kMoeMaxChoices || T * K > kMoeMaxSlots || D < 1 || H < 1 || E < 1 ||
+      E > kMoeMaxExperts || D > INT32_MAX / 64 || H > INT32_MAX / 64)
+    return false;
+  return (ceil_div(T * K, 128) + E) * ceil_div(std::max(D, H), 128) < (1 << 23);
+}
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+size_t nsh_op_moe_experts_state(int64_t T, int64_t K, int64_t D, int64_t H, int64_t E) {
+  return moe_shape_ok(T, K, D, H, E) && T > 0 ? experts_state_bytes({T, K, D, H, E}) : 0;
+}
+
+size_t nsh_op_moe_experts_workspace(int64_t T, int64_t K, int64_t D, int64_t H, int64_t E, int grad) {
+  return moe_shape_ok(T, K, D, H, E) && T > 0 ? experts_workspace_bytes({T, K, D, H, E}, grad != 0) : 0;
+}
+
+int nsh_op_moe_experts(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2,
+                       float* y, int64_t T, int64_t K, int64_t D, int64_t H, int64_t E, int act, void* state,
+                       void* workspace, void* stream) {
+  NSH_OP_REQUIRE(moe_shape_ok(T, K, D, H, E) && act >= 0 && act <= kActGelu && aligned16(state) &&
+                     aligned16(workspace) && (T == 0 || (x && idx && weight && W1 && W2 && y && workspace)),
+                 "moe_experts");
+  if (!stream_here((hipStream_t)stream, "moe_experts")) return -1;
+  if (T == 0) return 0;
+  return launch_experts(x, idx, weight, W1, W2, y, {T, K, D, H, E}, act, state, workspace, (hipStream_t)stream);
+}
+
+int nsh_op_moe_experts_grad(const float* dy, const float* x, const float* weight, const float* W1, const float* W2,
+                            const void* state, float* dx, float* dweight, float* dW1, float* dW2, int64_t T,
+                            int64_t K, int64_t D, int64_t H, int64_t E, int act, void* workspace, void* stream) {
+  NSH_OP_REQUIRE(moe_shape_ok(T, K, D, H, E) && act >= 0 && act <= kActGelu && aligned16(state) &&
+                     aligned16(workspace) && (T == 0 || (dy && x && weight && W1 && W2 && state && workspace)),
+                 "moe_experts_grad");
+  if (!stream_here((hipStream_t)stream, "moe_experts_grad")) return -1;
+  return launch_experts_grad(dy, x, weight, W1, W2, state, dx, dweight, dW1, dW2, {T, K, D, H, E}, act, workspace,
+                             (hipStream_t)stream);
+}
+
+// Sizes that the products' tiles and grids can index.
+static bool ns_shape_ok(int64_t n, int64_t r, int64_t c) {
+  return n >= 0 && n <= 65535 && r >= 1 && c >= 1 && std::min(r, c) <= 32768 && std::max(r, c) <= (1 << 22);
+}
+
+size_t nsh_op_newton_schulz_workspace(int64_t n, int64_t r, int64_t c) {
+  return ns_shape_ok(n, r, c) ? newton_schulz_bytes(n, r, c) : 0;
+}
+
+int nsh_op_newton_schulz(const float* g, float* q, int64_t n, int64_t r, int64_t c, int steps, void* workspace,
+                         void* stream) {
+  NSH_OP_REQUIRE(ns_shape_ok(n, r, c) && steps >= 0 && steps <= 100 && aligned16(workspace) &&
+                     (n == 0 || (g && q && workspace)),
+                 "newton_schulz");
+  if (!stream_here((hipStream_t)stream, "newton_schulz")) return -1;
+  return launch_newton_schulz(g, q, nullptr, n, r, c, steps, workspace, (hipStream_t)stream);
+}
+
+int nsh_op_muon_ns_step(float* w, const float* g, float* m, int64_t n, int64_t r, int64_t c, float lr, float mu,
+                        int nesterov, int steps, void* workspace, void* stream) {
+  NSH_OP_REQUIRE(ns_shape_ok(n, r, c) && steps >= 0 && steps <= 100 && aligned16(workspace) &&
+                     (n == 0 || (w && g && workspace)),
+                 "muon_ns_step");
+  if (!stream_here((hipStream_t)stream, "muon_ns_step")) return -1;
+  MuonNs step;
+  step.w = w; step.m = m; step.mu = mu; step.nesterov = nesterov != 0;
+  step.le = lr * sqrtf((float)std::min(r, c));
+  step.decay = 0.01f * lr;
+  return launch_newton_schulz(g, nullptr, &step, n, r, c, steps, workspace, (hipStream_t)stream);
+}
+
 }  // extern "C"

@@ -96,6 +96,15 @@ def lib():
             "nsh_op_embedding_grad": (ci, [vp, vp, vp, i64, i64, i64, vp]),
             "nsh_op_embedding_grad_noalloc": (ci, [vp, vp, vp, i64, i64, i64, vp]),
             "nsh_op_attention_fwd": (ci, [vp, vp, vp, vp, vp, i64, i64, i64]),
+            "nsh_op_moe_route": (ci, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, ci, ci, ci, cf, vp]),
+            "nsh_op_moe_route_grad": (ci, [vp, vp, vp, vp, vp, i64, i64, i64, ci, ci, cf, vp]),
+            "nsh_op_moe_experts_state": (sz, [i64, i64, i64, i64, i64]),
+            "nsh_op_moe_experts_workspace": (sz, [i64, i64, i64, i64, i64, ci]),
+            "nsh_op_moe_experts": (ci, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, ci, vp, vp, vp]),
+            "nsh_op_moe_experts_grad": (ci, [vp] * 10 + [i64, i64, i64, i64, i64, ci, vp, vp]),
+            "nsh_op_newton_schulz_workspace": (sz, [i64, i64, i64]),
+            "nsh_op_newton_schulz": (ci, [vp, vp, i64, i64, i64, ci, vp, vp]),
+            "nsh_op_muon_ns_step": (ci, [vp, vp, vp, i64, i64, i64, cf, cf, ci, ci, vp, vp]),
         }
         for name, (res, args) in sigs.items():
             fn = getattr(L, name)
