@@ -310,7 +310,8 @@ int nsh_op_moe_experts_grad(const float* dy, const float* x, const float* weight
  *   X = 3.4445 X + (-4.7750 A + 2.0315 A A) X   (X^T X where r > c)
  * g, q [n, r, c]; q may be g.  A matrix with an infinity or NaN comes out as
  * NaN, a zero one as zeros; the others of the batch are not touched by it.
- * n <= 65535, min(r, c) <= 32768, max(r, c) <= 2^22. */
+ * n <= 65535, min(r, c) <= 32768, max(r, c) <= 2^22, and n matrices of at most
+ * 2^22 blocks of 64 x 64 together. */
 size_t nsh_op_newton_schulz_workspace(int64_t n, int64_t r, int64_t c);
 int nsh_op_newton_schulz(const float* g, float* q, int64_t n, int64_t r, int64_t c, int steps, void* workspace,
                          void* stream);

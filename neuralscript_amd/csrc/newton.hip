@@ -1,11 +1,37 @@
 // Newton-Schulz orthogonalisation of n matrices [r, c], and the Muon step that
 // takes its update from it.
 //
-//   X = G / (|G|_F + 1e-7);  steps times: A = X X^T, X = a X + (b A + c A A) X
+//   X = G / (|G|_F + 1e-7);  steps times: S = X X^T, P = a I + b S + c S S, X = P X
 //
-// with X held wide ([m, N], m = min(r, c) <= N): each product drives every
-// singular value s in (0, 1] through a s + b s^3 + c s^5, which in five steps
-// ends between about 0.7 and 1.2 for all but the smallest.
+// with X held wide ([m, N], m = min(r, c) <= N): each step maps every singular
+// value s to a s + b s^3 + c s^5, which in five steps ends between about 0.7
+// and 1.2 for all but the smallest.
+//
+// Three products a step, m^2 N (half of a symmetric result), m^3 (half again)
+// and 2 m^2 N FLOP; bound by the matrix cores from some hundred rows on, below
+// by launches and the latency of a slab's loads.
+//
+// Products of two fp16 pieces.  The map keeps |X| and |S| (entries and singular
+// values) below 1.21^2 and |P| below 3.45 whatever G is, so one power of two
+// per operand puts every entry into fp16's range, and v = h + l with h =
+// fp16(v), l = fp16(v - h) holds 22 bits of it (23 with l's sign): two fp16
+// MFMA operands instead of split3.h's three bf16 ones, and three products h h,
+// h l, l h instead of six.  What that drops: 2^-23 of an operand at most (fp32:
+// 2^-24), l l below 2^-22 of a product, and of entries below 2^-18 the bits
+// under 2^-40.  Rounding at random, that is 2^-23.6 of a product, against the
+// 10 x 2^-24 and more that fp32 sums of 1024 terms lose; measured errors are
+// in the table of launch_newton_schulz.
+//
+// The norm's 1e-7 leaves X0 small where G is.  X is then held times 2^e, e = e0 -
+// 2 k at step k and not below 0 (a step grows X by at most 3.4445), so that its
+// entries keep their bits.
+//
+// Layout.  An operand with rows R and contraction length K is stored as
+// [piece][K / 8][R][8]: the 16-byte chunk of 8 consecutive k of one row is what
+// one lane of an MFMA takes, and a slab of a tile is contiguous runs of chunks,
+// copied to LDS as they lie.  K is padded with zeros to a multiple of 64.  X is
+// kept both ways, as the Gram product's operand (rows m, contraction N) and as
+// the update's (rows N, contraction m); S and P are symmetric and need one.
 #include <algorithm>
 
 #include "common.h"
@@ -14,9 +40,260 @@
 namespace nship {
 namespace {
 
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
 constexpr double kNsEps = 1e-7;
 constexpr int kNormParts = 64;  // partial sums of a matrix's norm
+// the operands' powers of two: X and S below 2 x 2^15 = fp16's range, P below 4 x 2^14
+constexpr float kUpX = 0x1p15f, kUpS = 0x1p15f, kUpP = 0x1p14f;
+
+__device__ __forceinline__ void split2(float v, _Float16& h, _Float16& l) {
+  h = (_Float16)v;
+  l = (_Float16)(v - (float)h);
+}
+
+// What a product is for, i.e. its epilogue.
+enum NsMode : int { kGram = 0, kPoly, kUpdate, kLast };
+
+struct NsArgs {
+  const _Float16* A;   // rows ra, contraction k (a multiple of 64)
+  const _Float16* B;   // rows rb
+  int64_t ra, rb, k;
+  int64_t sA, sB;      // matrix to matrix, halves
+  int tiles_m, tiles_n, tiles;  // of a matrix (symmetric: its lower triangle)
+  int n;
+  _Float16* out;       // kGram: S, kPoly: P, kUpdate: X as the Gram's operand [.][kout2 / 8][ra][8]
+  _Float16* out2;      // kUpdate: X as the update's operand [.][kout / 8][rb][8]
+  const _Float16* S;   // kPoly
+  int64_t sOut, sOut2;
+  int64_t kout, kout2; // padded contraction lengths of the outputs: of rows ra as k, of rows rb as k
+  float* f;            // kLast: q or w [ra][rb] per matrix
+  float le, decay;
+  int weights;         // kLast: f = f - le x - decay f
+  const int* ex;       // e0 of every matrix
+  int step;
+};
+
+__device__ __forceinline__ int ns_xcd_linear(int b, int T) {
+  const int per = T >> 3, rem = T & 7, x = b & 7, i = b >> 3;
+  return x * per + (x < rem ? x : rem) + i;
+}
+
+// One tile of C = A B^T: WM x WN waves of TM x TN blocks of 32x32, slabs of KS.
+template <int MODE, int WM, int WN, int TM, int TN, int KS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void ns_gemm_kernel(NsArgs g) {
+  constexpr int NT = 64 * WM * WN, RA = 32 * WM * TM, RB = 32 * WN * TN, OCT = KS / 8;
+  constexpr int CA = 2 * OCT * RA / NT, CB = 2 * OCT * RB / NT;  // chunks a thread
+  constexpr int kBuf = 2 * OCT * (RA + RB) * 16;
+  constexpr int kPitch = 40;  // halves of a transposing tile's row
+  constexpr int kTurn = 2 * 32 * kPitch * 2;
+  static_assert(CA * NT == 2 * OCT * RA && CB * NT == 2 * OCT * RB, "the chunks divide evenly");
+  static_assert(kTurn * WM * WN <= 2 * kBuf, "the transposing tiles fit");
+  constexpr bool kSym = MODE == kGram || MODE == kPoly;
+  __shared__ __attribute__((aligned(16))) char smem[2 * kBuf];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int wm = wave / WN, wn = wave % WN, l32 = lane & 31, kh = lane >> 5;
+  const int L = ns_xcd_linear(blockIdx.x, g.tiles * g.n);
+  const int mat = L / g.tiles;
+  int tm, tn = L % g.tiles;
+  if (kSym) {  // tile (tm, tn), tn <= tm, of a triangle counted by rows (RA == RB)
+    tm = (int)((sqrtf(8.f * (float)tn + 1.f) - 1.f) * 0.5f);
+    while ((int64_t)tm * (tm + 1) / 2 > tn) tm--;
+    while ((int64_t)(tm + 1) * (tm + 2) / 2 <= tn) tm++;
+    tn -= tm * (tm + 1) / 2;
+  } else {
+    tm = tn / g.tiles_n;
+    tn -= tm * g.tiles_n;
+  }
+  const int64_t m0 = (int64_t)tm * RA, n0 = (int64_t)tn * RB;
+  floatx16 acc[TM][TN];
+#pragma unroll
+  for (int r = 0; r < TM; r++)
+#pragma unroll
+    for (int c = 0; c < TN; c++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) acc[r][c][v] = 0.f;
+  {
+    // chunk i of thread t: (piece, octet, row), row fastest; rows past the end
+    // read the last one's (their results are not stored)
+    const uintx4* pa[CA];
+    const uintx4* pb[CB];
+#pragma unroll
+    for (int i = 0; i < CA; i++) {
+      const int c = t + NT * i, row = c % RA, o = c / RA % OCT, p = c / RA / OCT;
+      pa[i] = reinterpret_cast<const uintx4*>(g.A + mat * g.sA) + (p * (g.k / 8) + o) * g.ra +
+              min(m0 + row, g.ra - 1);
+    }
+#pragma unroll
+    for (int i = 0; i < CB; i++) {
+      const int c = t + NT * i, row = c % RB, o = c / RB % OCT, p = c / RB / OCT;
+      pb[i] = reinterpret_cast<const uintx4*>(g.B + mat * g.sB) + (p * (g.k / 8) + o) * g.rb +
+              min(n0 + row, g.rb - 1);
+    }
+    const int64_t stepa = OCT * g.ra, stepb = OCT * g.rb;
+    const int nk = (int)(g.k / KS);
+    uintx4 va[2][CA], vb[2][CB];
+    int next = 0;  // slab to load; past the last it is loaded again
+    auto load = [&](auto z) {
+      constexpr int Z = decltype(z)::value;
+#pragma unroll
+      for (int i = 0; i < CA; i++) va[Z][i] = *pa[i];
+#pragma unroll
+      for (int i = 0; i < CB; i++) vb[Z][i] = *pb[i];
+      const bool more = ++next < nk;
+#pragma unroll
+      for (int i = 0; i < CA; i++) pa[i] += more ? stepa : 0;
+#pragma unroll
+      for (int i = 0; i < CB; i++) pb[i] += more ? stepb : 0;
+    };
+    auto store = [&](auto z, char* to) {
+      constexpr int Z = decltype(z)::value;
+#pragma unroll
+      for (int i = 0; i < CA; i++) *reinterpret_cast<uintx4*>(to + (t + NT * i) * 16) = va[Z][i];
+#pragma unroll
+      for (int i = 0; i < CB; i++) *reinterpret_cast<uintx4*>(to + 2 * OCT * RA * 16 + (t + NT * i) * 16) = vb[Z][i];
+    };
+    using Even = std::integral_constant<int, 0>;
+    using Odd = std::integral_constant<int, 1>;
+    load(Even{});
+    load(Odd{});
+    store(Even{}, smem);
+    load(Even{});
+    __syncthreads();
+    auto slab = [&](int kt, auto z) {
+      const char* as = smem + (kt & 1) * kBuf + (kh * RA + wm * TM * 32 + l32) * 16;
+      const char* bs = smem + (kt & 1) * kBuf + 2 * OCT * RA * 16 + (kh * RB + wn * TN * 32 + l32) * 16;
+#pragma unroll
+      for (int s = 0; s < KS / 16; s++) {
+        half8 fa[TM][2], fb[TN][2];
+#pragma unroll
+        for (int c = 0; c < TN; c++)
+#pragma unroll
+          for (int p = 0; p < 2; p++)
+            fb[c][p] = *reinterpret_cast<const half8*>(bs + ((p * OCT + 2 * s) * RB + c * 32) * 16);
+#pragma unroll
+        for (int r = 0; r < TM; r++)
+#pragma unroll
+          for (int p = 0; p < 2; p++)
+            fa[r][p] = *reinterpret_cast<const half8*>(as + ((p * OCT + 2 * s) * RA + r * 32) * 16);
+#pragma unroll
+        for (int r = 0; r < TM; r++) {
+#pragma unroll
+          for (int c = 0; c < TN; c++)
+            acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[r][1], fb[c][0], acc[r][c], 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < TN; c++)
+            acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[r][0], fb[c][1], acc[r][c], 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < TN; c++)
+            acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[r][0], fb[c][0], acc[r][c], 0, 0, 0);
+        }
+      }
+      store(z, smem + ((kt + 1) & 1) * kBuf);
+      load(z);
+      __syncthreads();
+    };
+    for (int kt = 0; kt < nk; kt += 2) {
+      slab(kt, Odd{});
+      if (kt + 1 < nk) slab(kt + 1, Even{});
+    }
+  }
+  // Accumulator v of lane (l32, kh) in a 32x32 block: row 8 (v / 4) + 4 kh + v % 4, column l32.
+  const int64_t mw = m0 + wm * TM * 32, nw = n0 + wn * TN * 32;
+  const int ex = max(0, g.ex[mat] - 2 * g.step);  // X = 2^-ex times what is held
+  if constexpr (MODE == kLast) {
+    float* __restrict__ f = g.f + mat * g.ra * g.rb;
+    const float down = ldexpf(1.f / (kUpX * kUpP), -ex);
+#pragma unroll
+    for (int r = 0; r < TM; r++)
+#pragma unroll
+      for (int c = 0; c < TN; c++) {
+        const int64_t col = nw + c * 32 + l32;
+        if (col >= g.rb) continue;
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+          const int64_t row = mw + r * 32 + 8 * (v >> 2) + 4 * kh + (v & 3);
+          if (row >= g.ra) continue;
+          const float x = acc[r][c][v] * down;
+          float* p = f + row * g.rb + col;
+          *p = g.weights ? *p - g.le * x - g.decay * *p : x;
+        }
+      }
+    return;
+  } else {
+    // (S is held times 2^2ex)
+    const float by = MODE == kGram     ? kUpS / (kUpX * kUpX)
+                     : MODE == kUpdate ? ldexpf(1.f / kUpP, max(0, ex - 2) - ex)
+                                       : ldexpf(kNsC * kUpP / (kUpS * kUpS), -4 * ex);
+    const float bs = ldexpf(kNsB * kUpP / kUpS, -2 * ex);
+    char* turn = smem + wave * kTurn;
+    _Float16* __restrict__ out = g.out + mat * g.sOut;
+    _Float16* __restrict__ out2 = (kSym ? g.out : g.out2) + mat * (kSym ? g.sOut : g.sOut2);
+    const int64_t piece2 = g.kout * g.rb, piece = g.kout2 * g.ra;
+#pragma unroll
+    for (int r = 0; r < TM; r++)
+#pragma unroll
+      for (int c = 0; c < TN; c++) {
+        const int64_t row0 = mw + r * 32, col0 = nw + c * 32, col = col0 + l32;
+        // as [k = row][col]: four consecutive k of a column, half a chunk
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const int64_t k = row0 + 8 * q + 4 * kh;
+          const int64_t at = ((k / 8) * g.rb + col) * 8 + 4 * kh;
+          const bool in = col < g.rb && k < g.kout;
+          half4 h, l;
+          half4 sh = {0, 0, 0, 0}, sl = {0, 0, 0, 0};
+          if (MODE == kPoly && in) {  // (S is symmetric: its [k = row][col] is its (row, col))
+            const _Float16* s = g.S + mat * g.sOut + at;
+            sh = *reinterpret_cast<const half4*>(s);
+            sl = *reinterpret_cast<const half4*>(s + piece2);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            float x = acc[r][c][4 * q + u] * by;
+            if (MODE == kPoly)
+              x += (k + u == col ? kNsA * kUpP : 0.f) + bs * ((float)sh[u] + (float)sl[u]);
+            x = k + u < g.ra && col < g.rb ? x : 0.f;  // (padding)
+            _Float16 hh, ll;
+            split2(x, hh, ll);
+            h[u] = hh;
+            l[u] = ll;
+          }
+          if (in) {
+            *reinterpret_cast<half4*>(out2 + at) = h;
+            *reinterpret_cast<half4*>(out2 + piece2 + at) = l;
+          }
+          _Float16* to = reinterpret_cast<_Float16*>(turn) + (8 * q + 4 * kh) * kPitch + l32;
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            to[u * kPitch] = h[u];
+            to[u * kPitch + 32 * kPitch] = l[u];
+          }
+        }
+        if (kSym && tm == tn) continue;  // (the other way round lies in the same tile)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        // as [k = col][row]: a whole chunk of a row
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+          const int o = 2 * q + kh;
+          const int64_t row = row0 + l32, k = col0 + 8 * o;
+          const _Float16* from = reinterpret_cast<const _Float16*>(turn) + l32 * kPitch + 8 * o;
+          const half8 h = *reinterpret_cast<const half8*>(from);
+          const half8 l = *reinterpret_cast<const half8*>(from + 32 * kPitch);
+          if (row < g.ra && k < g.kout2) {
+            _Float16* to = out + ((k / 8) * g.ra + row) * 8;
+            *reinterpret_cast<half8*>(to) = h;
+            *reinterpret_cast<half8*>(to + piece) = l;
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+  }
+}
 
 __device__ __forceinline__ float update_of(float g, float m, float mu, int nesterov) {
   return nesterov ? g + mu * m : m;
@@ -44,36 +321,102 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const float* __restrict__ 
   if (threadIdx.x == 0) part[(int64_t)blockIdx.y * kNormParts + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
-// X [m, N] = the update over its norm, transposed where r > c.
-__global__ __launch_bounds__(256) void ns_start_kernel(const float* __restrict__ g, const float* __restrict__ m,
-                                                       float mu, int nesterov, int64_t r, int64_t c, int parts,
-                                                       const double* __restrict__ part, float* __restrict__ X) {
-  const int64_t elems = r * c, base = (int64_t)blockIdx.y * elems;
+// 1 / (|u|_F + 1e-7) from the partial sums; NaN where the norm is not finite,
+// so that the whole matrix is.
+__device__ __forceinline__ double ns_scale(const double* __restrict__ part, int parts, int* ex = nullptr) {
   double sq = 0.;
-  for (int p = 0; p < parts; p++) sq += part[(int64_t)blockIdx.y * kNormParts + p];
-  const double by = 1. / (sqrt(sq) + kNsEps);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elems; i += (int64_t)gridDim.x * 256) {
-    float u = g[base + i];
-    if (m) u = update_of(u, m[base + i], mu, nesterov);
-    const int64_t row = i / c, col = i - row * c;
-    X[base + (r > c ? col * r + row : i)] = (float)(u * by);
+  for (int p = 0; p < parts; p++) sq += part[p];
+  const double norm = sqrt(sq), by = sq < __builtin_inf() ? 1. / (norm + kNsEps) : __builtin_nan("");
+  // 2^ex |X0| in (1/2, 1]: |X0| is at least 1e-38, since no smaller float has a square here
+  if (ex) *ex = norm * by > 0. ? max(0, min(126, ilogb(1. / (norm * by)))) : 0;
+  return by;
+}
+
+// X = the update over its norm in both layouts, a tile of 64 x 64 of X a
+// workgroup: gram [.][Np / 8][m][8], upd [.][mp / 8][N][8].
+struct NsStart {
+  const float* g;
+  const float* m;
+  float mu;
+  int nesterov;
+  int64_t r, c;
+  int parts, tiles_n;
+  const double* part;
+  int* ex;
+  _Float16* gram;
+  _Float16* upd;
+  int64_t M, N, mp, np;
+};
+__global__ __launch_bounds__(256) void ns_start_kernel(NsStart a) {
+  __shared__ float x[64][65];  // [i][j] of X
+  const int64_t elems = a.r * a.c, base = (int64_t)blockIdx.y * elems;
+  int ex;
+  const double by = ns_scale(a.part + (int64_t)blockIdx.y * kNormParts, a.parts, &ex);
+  const double up = ldexp(by * kUpX, ex);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.ex[blockIdx.y] = ex;
+  const int64_t i0 = (int64_t)(blockIdx.x / a.tiles_n) * 64, j0 = (int64_t)(blockIdx.x % a.tiles_n) * 64;
+  const int t = threadIdx.x, lo = t & 63, hi = t >> 6;
+  const bool tall = a.r > a.c;
+#pragma unroll
+  for (int q = 0; q < 16; q++) {
+    const int h = hi + 4 * q;  // (lanes run along g's rows)
+    const int64_t i = i0 + (tall ? lo : h), j = j0 + (tall ? h : lo);
+    float u = 0.f;
+    if (i < a.M && j < a.N) {
+      const int64_t at = base + (tall ? j * a.c + i : i * a.c + j);
+      u = a.g[at];
+      if (a.m) u = update_of(u, a.m[at], a.mu, a.nesterov);
+      u = (float)(u * up);
+    }
+    if (tall) x[lo][h] = u;
+    else x[h][lo] = u;
+  }
+  __syncthreads();
+  const int64_t pg = a.np * a.M, pu = a.mp * a.N;
+  _Float16* __restrict__ gram = a.gram + blockIdx.y * 2 * pg;
+  _Float16* __restrict__ upd = a.upd + blockIdx.y * 2 * pu;
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    const int o = hi + 4 * q;
+    half8 h, l;
+    if (i0 + lo < a.M) {
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        _Float16 hh, ll;
+        split2(x[lo][8 * o + u], hh, ll);
+        h[u] = hh;
+        l[u] = ll;
+      }
+      _Float16* to = gram + ((j0 / 8 + o) * a.M + i0 + lo) * 8;
+      *reinterpret_cast<half8*>(to) = h;
+      *reinterpret_cast<half8*>(to + pg) = l;
+    }
+    if (j0 + lo < a.N) {
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        _Float16 hh, ll;
+        split2(x[8 * o + u][lo], hh, ll);
+        h[u] = hh;
+        l[u] = ll;
+      }
+      _Float16* to = upd + ((i0 / 8 + o) * a.N + j0 + lo) * 8;
+      *reinterpret_cast<half8*>(to) = h;
+      *reinterpret_cast<half8*>(to + pu) = l;
+    }
   }
 }
 
-// P = a I + b A + c P
-__global__ __launch_bounds__(256) void ns_poly_kernel(const float* __restrict__ A, float* __restrict__ P, int64_t m) {
-  const int64_t elems = m * m, base = (int64_t)blockIdx.y * elems;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elems; i += (int64_t)gridDim.x * 256)
-    P[base + i] = (i / m == i % m ? kNsA : 0.f) + kNsB * A[base + i] + kNsC * P[base + i];
-}
-
-__global__ __launch_bounds__(256) void ns_end_kernel(const float* __restrict__ X, float* __restrict__ q,
-                                                     float* __restrict__ w, float le, float decay, int64_t r,
-                                                     int64_t c) {
-  const int64_t elems = r * c, base = (int64_t)blockIdx.y * elems;
+// No steps: the update over its norm itself.
+__global__ __launch_bounds__(256) void ns_normalise_kernel(const float* g, const float* __restrict__ m, float mu,
+                                                           int nesterov, int64_t elems, int parts,
+                                                           const double* __restrict__ part, float* q,
+                                                           float* __restrict__ w, float le, float decay) {
+  const int64_t base = (int64_t)blockIdx.y * elems;
+  const double by = ns_scale(part + (int64_t)blockIdx.y * kNormParts, parts);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elems; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / c, col = i - row * c;
-    const float x = X[base + (r > c ? col * r + row : i)];
+    float u = g[base + i];
+    if (m) u = update_of(u, m[base + i], mu, nesterov);
+    const float x = (float)(u * by);
     if (w) w[base + i] = w[base + i] - le * x - decay * w[base + i];
     else q[base + i] = x;
   }
@@ -81,59 +424,113 @@ __global__ __launch_bounds__(256) void ns_end_kernel(const float* __restrict__ X
 
 constexpr int64_t round64(int64_t n) { return (n + 63) / 64 * 64; }
 
+struct NsSizes {
+  int64_t m, N, mp, np, gram, upd, sym;  // halves of a matrix's operands
+  NsSizes(int64_t r, int64_t c) {
+    m = std::min(r, c);
+    N = std::max(r, c);
+    mp = round64(m);
+    np = round64(N);
+    gram = 2 * np * m;
+    upd = 2 * mp * N;
+    sym = 2 * mp * m;
+  }
+};
+
+template <int MODE>
+int launch_product(NsArgs& g, hipStream_t s) {
+  constexpr bool kSym = MODE == kGram || MODE == kPoly;
+  auto tiles = [&](int64_t bm, int64_t bn) {
+    g.tiles_m = (int)ceil_div(g.ra, bm);
+    g.tiles_n = (int)ceil_div(g.rb, bn);
+    const int64_t t = kSym ? (int64_t)g.tiles_m * (g.tiles_m + 1) / 2 : (int64_t)g.tiles_m * g.tiles_n;
+    g.tiles = (int)t;
+    return t * g.n;
+  };
+  if (tiles(256, 256) >= 256)
+    hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 4, 4, 2, 16>), dim3((unsigned)(g.tiles * (int64_t)g.n)), dim3(512), 0, s, g);
+  else if (tiles(128, 128) >= 256)
+    hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 2, 2, 2, 32>), dim3((unsigned)(g.tiles * (int64_t)g.n)), dim3(256), 0, s, g);
+  else {
+    tiles(64, 64);
+    hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 2, 1, 1, 64>), dim3((unsigned)(g.tiles * (int64_t)g.n)), dim3(256), 0, s, g);
+  }
+  NSH_LAUNCHED();
+  return 0;
+}
+
 }  // namespace
 
-// the norms' partial sums, X twice, A and P
+// the norms' partial sums; their exponents; X as the Gram's operand, twice as the update's; S and P
 size_t newton_schulz_bytes(int64_t n, int64_t r, int64_t c) {
-  const int64_t m = std::min(r, c);
-  return (size_t)n * kNormParts * 8 + 4 * (size_t)(2 * round64(n * r * c) + 2 * round64(n * m * m));
+  const NsSizes z(r, c);
+  return (size_t)round64(n) * 4 + (size_t)n * (kNormParts * 8 + 2 * (size_t)(z.gram + 2 * z.upd + 2 * z.sym));
 }
 
 int launch_newton_schulz(const float* g, float* q, const MuonNs* step, int64_t n, int64_t r, int64_t c, int steps,
                          void* workspace, hipStream_t s) {
-  const int64_t m = std::min(r, c), N = std::max(r, c), elems = r * c;
+  const NsSizes z(r, c);
+  const int64_t elems = r * c;
   if (n <= 0 || elems <= 0) return 0;
   double* part = static_cast<double*>(workspace);
-  float* X = reinterpret_cast<float*>(part + n * kNormParts);
-  float* Y = X + round64(n * elems);
-  float* A = Y + round64(n * elems);
-  float* P = A + round64(n * m * m);
+  int* ex = reinterpret_cast<int*>(part + n * kNormParts);
+  _Float16* gram = reinterpret_cast<_Float16*>(ex + round64(n));
+  _Float16* upd = gram + n * z.gram;
+  _Float16* upd2 = upd + n * z.upd;
+  _Float16* S = upd2 + n * z.upd;
+  _Float16* P = S + n * z.sym;
   const int parts = (int)std::min<int64_t>(kNormParts, ceil_div(elems, 1024));
   float* mom = step ? step->m : nullptr;
   const float mu = step ? step->mu : 0.f;
   const int nesterov = step ? step->nesterov : 0;
-  const dim3 all((unsigned)std::min<int64_t>(ceil_div(elems, 1024), 4096), (unsigned)n);
   hipLaunchKernelGGL(ns_norm_kernel, dim3(parts, (unsigned)n), dim3(256), 0, s, g, mom, mu, nesterov, elems, part);
   NSH_LAUNCHED();
-  hipLaunchKernelGGL(ns_start_kernel, all, dim3(256), 0, s, g, mom, mu, nesterov, r, c, parts, part, X);
+  if (steps == 0) {
+    hipLaunchKernelGGL(ns_normalise_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(elems, 1024), 4096), (unsigned)n),
+                       dim3(256), 0, s, g, mom, mu, nesterov, elems, parts, part, q, step ? step->w : nullptr,
+                       step ? step->le : 0.f, step ? step->decay : 0.f);
+    NSH_LAUNCHED();
+    return 0;
+  }
+  NsStart a;
+  a.g = g; a.m = mom; a.mu = mu; a.nesterov = nesterov;
+  a.r = r; a.c = c;
+  a.parts = parts; a.part = part; a.ex = ex;
+  a.gram = gram; a.upd = upd;
+  a.M = z.m; a.N = z.N; a.mp = z.mp; a.np = z.np;
+  a.tiles_n = (int)(z.np / 64);
+  hipLaunchKernelGGL(ns_start_kernel, dim3((unsigned)(z.mp / 64 * (z.np / 64)), (unsigned)n), dim3(256), 0, s, a);
   NSH_LAUNCHED();
   for (int k = 0; k < steps; k++) {
-    GemmArgs a;
-    a.A = X; a.B = X; a.C = A;
-    a.M = (int)m; a.N = (int)m; a.K = (int)N;
-    a.lda = N; a.ldb = N; a.ldc = m;
-    a.sA = elems; a.sB = elems; a.sC = m * m;
-    if (launch_gemm_ex(a, false, true, (int)n, s) != 0) return -1;
-    GemmArgs p;
-    p.A = A; p.B = A; p.C = P;
-    p.M = (int)m; p.N = (int)m; p.K = (int)m;
-    p.lda = m; p.ldb = m; p.ldc = m;
-    p.sA = m * m; p.sB = m * m; p.sC = m * m;
-    if (launch_gemm_ex(p, false, false, (int)n, s) != 0) return -1;
-    hipLaunchKernelGGL(ns_poly_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(m * m, 1024), 4096), (unsigned)n),
-                       dim3(256), 0, s, A, P, m);
-    NSH_LAUNCHED();
-    GemmArgs x;
-    x.A = P; x.B = X; x.C = Y;
-    x.M = (int)m; x.N = (int)N; x.K = (int)m;
-    x.lda = m; x.ldb = N; x.ldc = N;
-    x.sA = m * m; x.sB = elems; x.sC = elems;
-    if (launch_gemm_ex(x, false, false, (int)n, s) != 0) return -1;
-    std::swap(X, Y);
+    NsArgs p{};
+    p.n = (int)n;
+    p.ex = ex; p.step = k;
+    p.A = p.B = gram;
+    p.ra = p.rb = z.m; p.k = z.np;
+    p.sA = p.sB = z.gram;
+    p.out = S; p.sOut = z.sym;
+    p.kout = p.kout2 = z.mp;
+    if (launch_product<kGram>(p, s) != 0) return -1;
+    p.A = p.B = S; p.k = z.mp;
+    p.sA = p.sB = z.sym;
+    p.S = S; p.out = P;
+    if (launch_product<kPoly>(p, s) != 0) return -1;
+    const bool last = k + 1 == steps, tall = last && r > c;
+    p.A = tall ? upd : P; p.sA = tall ? z.upd : z.sym; p.ra = tall ? z.N : z.m;
+    p.B = tall ? P : upd; p.sB = tall ? z.sym : z.upd; p.rb = tall ? z.m : z.N;
+    p.k = z.mp;
+    if (last) {
+      p.f = step ? step->w : q;
+      p.weights = step != nullptr;
+      p.le = step ? step->le : 0.f;
+      p.decay = step ? step->decay : 0.f;
+      return launch_product<kLast>(p, s);
+    }
+    p.out = gram; p.sOut = z.gram; p.kout2 = z.np;
+    p.out2 = upd2; p.sOut2 = z.upd; p.kout = z.mp;
+    if (launch_product<kUpdate>(p, s) != 0) return -1;
+    std::swap(upd, upd2);
   }
-  hipLaunchKernelGGL(ns_end_kernel, all, dim3(256), 0, s, X, q, step ? step->w : nullptr, step ? step->le : 0.f,
-                     step ? step->decay : 0.f, r, c);
-  NSH_LAUNCHED();
   return 0;
 }
 

@@ -2204,7 +2204,8 @@ int nsh_op_moe_experts_grad(const float* dy, const float* x, const float* weight
 
 // Sizes that the products' tiles and grids can index.
 static bool ns_shape_ok(int64_t n, int64_t r, int64_t c) {
-  return n >= 0 && n <= 65535 && r >= 1 && c >= 1 && std::min(r, c) <= 32768 && std::max(r, c) <= (1 << 22);
+  return n >= 0 && n <= 65535 && r >= 1 && c >= 1 && std::min(r, c) <= 32768 && std::max(r, c) <= (1 << 22) &&
+         n * (ceil_div(r, 64) * ceil_div(c, 64)) <= (1 << 22);
 }
 
 size_t nsh_op_newton_schulz_workspace(int64_t n, int64_t r, int64_t c) {

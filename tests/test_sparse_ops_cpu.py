@@ -111,6 +111,8 @@ def test_newton_schulz_refuses_two_large_sides():
     a[3] = a[4] = 32769
     refused("newton_schulz", a)
     assert runtime.lib().nsh_op_newton_schulz_workspace(2, 32769, 32769) == 0
+    a[2:5] = [17, 32768, 32768]  # more blocks than a grid holds
+    refused("newton_schulz", a)
 
 
 def test_empty_calls_succeed():
