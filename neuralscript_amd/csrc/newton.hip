@@ -29,7 +29,7 @@
 // Layout.  An operand with rows R and contraction length K is stored as
 // [piece][K / 8][R][8]: the 16-byte chunk of 8 consecutive k of one row is what
 // one lane of an MFMA takes, and a slab of a tile is contiguous runs of chunks,
-// copied to LDS as they lie.  K is padded with zeros to a multiple of 64.  X is
+// copied to LDS as they lie.  K is padded with zeros to a multiple of 32.  X is
 // kept both ways, as the Gram product's operand (rows m, contraction N) and as
 // the update's (rows N, contraction m); S and P are symmetric and need one.
 #include <algorithm>
@@ -41,6 +41,7 @@ namespace nship {
 namespace {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
@@ -60,7 +61,7 @@ __device__ __forceinline__ void split2(float v, _Float16& h, _Float16& l) {
 enum NsMode : int { kGram = 0, kPoly, kUpdate, kLast };
 
 struct NsArgs {
-  const _Float16* A;   // rows ra, contraction k (a multiple of 64)
+  const _Float16* A;   // rows ra, contraction k (a multiple of 32)
   const _Float16* B;   // rows rb
   int64_t ra, rb, k;
   int64_t sA, sB;      // matrix to matrix, halves
@@ -83,32 +84,137 @@ __device__ __forceinline__ int ns_xcd_linear(int b, int T) {
   return x * per + (x < rem ? x : rem) + i;
 }
 
+// Tile of linear index t: by rows, or of a lower triangle (tn <= tm) by rows.
+template <bool SYM>
+__device__ __forceinline__ void ns_tile(int t, int tiles_n, int& tm, int& tn) {
+  if (SYM) {
+    tm = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while ((int64_t)tm * (tm + 1) / 2 > t) tm--;
+    while ((int64_t)(tm + 1) * (tm + 2) / 2 <= t) tm++;
+    tn = t - tm * (tm + 1) / 2;
+  } else {
+    tm = t / tiles_n;
+    tn = t - tm * tiles_n;
+  }
+}
+
+constexpr int kPitch = 40;                       // halves of a transposing tile's row
+constexpr int kTurnBytes = 2 * 32 * kPitch * 2;  // of a wave's transposing tile
+
+// One wave's TM x TN blocks of 32x32 from (mw, nw), by what the product is for.
+// turn: kTurnBytes of LDS of the wave's own.  diagonal: a symmetric result's
+// tile on the diagonal.
+template <int MODE, int TM, int TN>
+__device__ __forceinline__ void ns_epilogue(const NsArgs& g, const floatx16 (&acc)[TM][TN], char* turn, int mat,
+                                            int64_t mw, int64_t nw, int l32, int kh, bool diagonal) {
+  constexpr bool kSym = MODE == kGram || MODE == kPoly;
+  // Accumulator v of lane (l32, kh) in a 32x32 block: row 8 (v / 4) + 4 kh + v % 4, column l32.
+  const int ex = max(0, g.ex[mat] - 2 * g.step);  // X = 2^-ex times what is held
+  if constexpr (MODE == kLast) {
+    float* __restrict__ f = g.f + mat * g.ra * g.rb;
+    const float down = ldexpf(1.f / (kUpX * kUpP), -ex);
+#pragma unroll
+    for (int r = 0; r < TM; r++)
+#pragma unroll
+      for (int c = 0; c < TN; c++) {
+        const int64_t col = nw + c * 32 + l32;
+        if (col >= g.rb) continue;
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+          const int64_t row = mw + r * 32 + 8 * (v >> 2) + 4 * kh + (v & 3);
+          if (row >= g.ra) continue;
+          const float x = acc[r][c][v] * down;
+          float* p = f + row * g.rb + col;
+          *p = g.weights ? *p - g.le * x - g.decay * *p : x;
+        }
+      }
+    return;
+  } else {
+    // (S is held times 2^2ex)
+    const float by = MODE == kGram     ? kUpS / (kUpX * kUpX)
+                     : MODE == kUpdate ? ldexpf(1.f / kUpP, max(0, ex - 2) - ex)
+                                       : ldexpf(kNsC * kUpP / (kUpS * kUpS), -4 * ex);
+    const float bs = ldexpf(kNsB * kUpP / kUpS, -2 * ex);
+    _Float16* __restrict__ out = g.out + mat * g.sOut;
+    _Float16* __restrict__ out2 = (kSym ? g.out : g.out2) + mat * (kSym ? g.sOut : g.sOut2);
+    const int64_t piece2 = g.kout * g.rb, piece = g.kout2 * g.ra;
+#pragma unroll
+    for (int r = 0; r < TM; r++)
+#pragma unroll
+      for (int c = 0; c < TN; c++) {
+        const int64_t row0 = mw + r * 32, col0 = nw + c * 32, col = col0 + l32;
+        // as [k = row][col]: four consecutive k of a column, half a chunk
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const int64_t k = row0 + 8 * q + 4 * kh;
+          const int64_t at = ((k / 8) * g.rb + col) * 8 + 4 * kh;
+          const bool in = col < g.rb && k < g.kout;
+          half4 h, l;
+          half4 sh = {0, 0, 0, 0}, sl = {0, 0, 0, 0};
+          if (MODE == kPoly && in) {  // (S is symmetric: its [k = row][col] is its (row, col))
+            const _Float16* s = g.S + mat * g.sOut + at;
+            sh = *reinterpret_cast<const half4*>(s);
+            sl = *reinterpret_cast<const half4*>(s + piece2);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            float x = acc[r][c][4 * q + u] * by;
+            if (MODE == kPoly)
+              x += (k + u == col ? kNsA * kUpP : 0.f) + bs * ((float)sh[u] + (float)sl[u]);
+            x = k + u < g.ra && col < g.rb ? x : 0.f;  // (padding)
+            _Float16 hh, ll;
+            split2(x, hh, ll);
+            h[u] = hh;
+            l[u] = ll;
+          }
+          if (in) {
+            *reinterpret_cast<half4*>(out2 + at) = h;
+            *reinterpret_cast<half4*>(out2 + piece2 + at) = l;
+          }
+          _Float16* to = reinterpret_cast<_Float16*>(turn) + (8 * q + 4 * kh) * kPitch + l32;
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            to[u * kPitch] = h[u];
+            to[u * kPitch + 32 * kPitch] = l[u];
+          }
+        }
+        if (diagonal) continue;  // (the other way round lies in the same tile)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        // as [k = col][row]: a whole chunk of a row
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+          const int o = 2 * q + kh;
+          const int64_t row = row0 + l32, k = col0 + 8 * o;
+          const _Float16* from = reinterpret_cast<const _Float16*>(turn) + l32 * kPitch + 8 * o;
+          const half8 h = *reinterpret_cast<const half8*>(from);
+          const half8 l = *reinterpret_cast<const half8*>(from + 32 * kPitch);
+          if (row < g.ra && k < g.kout2) {
+            _Float16* to = out + ((k / 8) * g.ra + row) * 8;
+            *reinterpret_cast<half8*>(to) = h;
+            *reinterpret_cast<half8*>(to + piece) = l;
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+  }
+}
+
 // One tile of C = A B^T: WM x WN waves of TM x TN blocks of 32x32, slabs of KS.
 template <int MODE, int WM, int WN, int TM, int TN, int KS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void ns_gemm_kernel(NsArgs g) {
   constexpr int NT = 64 * WM * WN, RA = 32 * WM * TM, RB = 32 * WN * TN, OCT = KS / 8;
   constexpr int CA = 2 * OCT * RA / NT, CB = 2 * OCT * RB / NT;  // chunks a thread
   constexpr int kBuf = 2 * OCT * (RA + RB) * 16;
-  constexpr int kPitch = 40;  // halves of a transposing tile's row
-  constexpr int kTurn = 2 * 32 * kPitch * 2;
   static_assert(CA * NT == 2 * OCT * RA && CB * NT == 2 * OCT * RB, "the chunks divide evenly");
-  static_assert(kTurn * WM * WN <= 2 * kBuf, "the transposing tiles fit");
+  static_assert(kTurnBytes * WM * WN <= 2 * kBuf, "the transposing tiles fit");
   constexpr bool kSym = MODE == kGram || MODE == kPoly;
   __shared__ __attribute__((aligned(16))) char smem[2 * kBuf];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int wm = wave / WN, wn = wave % WN, l32 = lane & 31, kh = lane >> 5;
   const int L = ns_xcd_linear(blockIdx.x, g.tiles * g.n);
   const int mat = L / g.tiles;
-  int tm, tn = L % g.tiles;
-  if (kSym) {  // tile (tm, tn), tn <= tm, of a triangle counted by rows (RA == RB)
-    tm = (int)((sqrtf(8.f * (float)tn + 1.f) - 1.f) * 0.5f);
-    while ((int64_t)tm * (tm + 1) / 2 > tn) tm--;
-    while ((int64_t)(tm + 1) * (tm + 2) / 2 <= tn) tm++;
-    tn -= tm * (tm + 1) / 2;
-  } else {
-    tm = tn / g.tiles_n;
-    tn -= tm * g.tiles_n;
-  }
+  int tm, tn;
+  ns_tile<kSym>(L % g.tiles, g.tiles_n, tm, tn);
   const int64_t m0 = (int64_t)tm * RA, n0 = (int64_t)tn * RB;
   floatx16 acc[TM][TN];
 #pragma unroll
@@ -202,97 +308,82 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_gemm_kernel(NsArgs g) {
       if (kt + 1 < nk) slab(kt + 1, Even{});
     }
   }
-  // Accumulator v of lane (l32, kh) in a 32x32 block: row 8 (v / 4) + 4 kh + v % 4, column l32.
-  const int64_t mw = m0 + wm * TM * 32, nw = n0 + wn * TN * 32;
-  const int ex = max(0, g.ex[mat] - 2 * g.step);  // X = 2^-ex times what is held
-  if constexpr (MODE == kLast) {
-    float* __restrict__ f = g.f + mat * g.ra * g.rb;
-    const float down = ldexpf(1.f / (kUpX * kUpP), -ex);
+  ns_epilogue<MODE, TM, TN>(g, acc, smem + wave * kTurnBytes, mat, m0 + wm * TM * 32, n0 + wn * TN * 32, l32, kh,
+                            kSym && tm == tn);
+}
+
+// The same product where larger tiles leave most CUs idle: 32 x 32 outputs a
+// workgroup, whose K is dealt out in 16-steps to eight waves that take their
+// operands straight into registers, kFewU steps at a time and without barriers;
+// the eight sums meet in LDS.  Bound by what a CU can pull from the L2 (64 rows
+// of K a tile) and its one or two round trips.  Measured and not kept: 64 x 64
+// tiles with K dealt out to four waves of each 32 x 32 block (fewer CUs pull
+// more; 3 of 1000 x 333: Gram product 15 us).
+constexpr int kFewU = 8;
+template <int MODE>
+__global__ __launch_bounds__(512) void ns_few_kernel(NsArgs g) {
+  constexpr bool kSym = MODE == kGram || MODE == kPoly;
+  __shared__ __attribute__((aligned(16))) float part[7][1024];
+  const int t = threadIdx.x, lane = t & 63, l32 = lane & 31, kh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int L = ns_xcd_linear(blockIdx.x, g.tiles * g.n);
+  const int mat = L / g.tiles;
+  int tm, tn;
+  ns_tile<kSym>(L % g.tiles, g.tiles_n, tm, tn);
+  const int64_t mw = (int64_t)tm * 32, nw = (int64_t)tn * 32;
+  floatx16 acc;
 #pragma unroll
-    for (int r = 0; r < TM; r++)
+  for (int v = 0; v < 16; v++) acc[v] = 0.f;
+  {
+    // chunk (piece, octet 2 s + kh, row) of step s
+    const half8* pa = reinterpret_cast<const half8*>(g.A + mat * g.sA) + kh * g.ra + min(mw + l32, g.ra - 1);
+    const half8* pb = reinterpret_cast<const half8*>(g.B + mat * g.sB) + kh * g.rb + min(nw + l32, g.rb - 1);
+    const int64_t la = g.k / 8 * g.ra, lb = g.k / 8 * g.rb;  // to the other piece
+    const int all = (int)(g.k / 16);
+    // steps s, s + 8, .. of this wave
+    auto steps = [&](int s0, auto count) {
+      constexpr int CNT = decltype(count)::value;
+      half8 a[CNT][2], b[CNT][2];
 #pragma unroll
-      for (int c = 0; c < TN; c++) {
-        const int64_t col = nw + c * 32 + l32;
-        if (col >= g.rb) continue;
-#pragma unroll
-        for (int v = 0; v < 16; v++) {
-          const int64_t row = mw + r * 32 + 8 * (v >> 2) + 4 * kh + (v & 3);
-          if (row >= g.ra) continue;
-          const float x = acc[r][c][v] * down;
-          float* p = f + row * g.rb + col;
-          *p = g.weights ? *p - g.le * x - g.decay * *p : x;
-        }
+      for (int u = 0; u < CNT; u++) {
+        const int64_t o = 2 * ((int64_t)s0 + 8 * u);
+        a[u][0] = pa[o * g.ra];
+        a[u][1] = pa[o * g.ra + la];
+        b[u][0] = pb[o * g.rb];
+        b[u][1] = pb[o * g.rb + lb];
       }
-    return;
-  } else {
-    // (S is held times 2^2ex)
-    const float by = MODE == kGram     ? kUpS / (kUpX * kUpX)
-                     : MODE == kUpdate ? ldexpf(1.f / kUpP, max(0, ex - 2) - ex)
-                                       : ldexpf(kNsC * kUpP / (kUpS * kUpS), -4 * ex);
-    const float bs = ldexpf(kNsB * kUpP / kUpS, -2 * ex);
-    char* turn = smem + wave * kTurn;
-    _Float16* __restrict__ out = g.out + mat * g.sOut;
-    _Float16* __restrict__ out2 = (kSym ? g.out : g.out2) + mat * (kSym ? g.sOut : g.sOut2);
-    const int64_t piece2 = g.kout * g.rb, piece = g.kout2 * g.ra;
 #pragma unroll
-    for (int r = 0; r < TM; r++)
-#pragma unroll
-      for (int c = 0; c < TN; c++) {
-        const int64_t row0 = mw + r * 32, col0 = nw + c * 32, col = col0 + l32;
-        // as [k = row][col]: four consecutive k of a column, half a chunk
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          const int64_t k = row0 + 8 * q + 4 * kh;
-          const int64_t at = ((k / 8) * g.rb + col) * 8 + 4 * kh;
-          const bool in = col < g.rb && k < g.kout;
-          half4 h, l;
-          half4 sh = {0, 0, 0, 0}, sl = {0, 0, 0, 0};
-          if (MODE == kPoly && in) {  // (S is symmetric: its [k = row][col] is its (row, col))
-            const _Float16* s = g.S + mat * g.sOut + at;
-            sh = *reinterpret_cast<const half4*>(s);
-            sl = *reinterpret_cast<const half4*>(s + piece2);
-          }
-#pragma unroll
-          for (int u = 0; u < 4; u++) {
-            float x = acc[r][c][4 * q + u] * by;
-            if (MODE == kPoly)
-              x += (k + u == col ? kNsA * kUpP : 0.f) + bs * ((float)sh[u] + (float)sl[u]);
-            x = k + u < g.ra && col < g.rb ? x : 0.f;  // (padding)
-            _Float16 hh, ll;
-            split2(x, hh, ll);
-            h[u] = hh;
-            l[u] = ll;
-          }
-          if (in) {
-            *reinterpret_cast<half4*>(out2 + at) = h;
-            *reinterpret_cast<half4*>(out2 + piece2 + at) = l;
-          }
-          _Float16* to = reinterpret_cast<_Float16*>(turn) + (8 * q + 4 * kh) * kPitch + l32;
-#pragma unroll
-          for (int u = 0; u < 4; u++) {
-            to[u * kPitch] = h[u];
-            to[u * kPitch + 32 * kPitch] = l[u];
-          }
-        }
-        if (kSym && tm == tn) continue;  // (the other way round lies in the same tile)
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        // as [k = col][row]: a whole chunk of a row
-#pragma unroll
-        for (int q = 0; q < 2; q++) {
-          const int o = 2 * q + kh;
-          const int64_t row = row0 + l32, k = col0 + 8 * o;
-          const _Float16* from = reinterpret_cast<const _Float16*>(turn) + l32 * kPitch + 8 * o;
-          const half8 h = *reinterpret_cast<const half8*>(from);
-          const half8 l = *reinterpret_cast<const half8*>(from + 32 * kPitch);
-          if (row < g.ra && k < g.kout2) {
-            _Float16* to = out + ((k / 8) * g.ra + row) * 8;
-            *reinterpret_cast<half8*>(to) = h;
-            *reinterpret_cast<half8*>(to + piece) = l;
-          }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      for (int u = 0; u < CNT; u++) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][1], b[u][0], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][0], b[u][1], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][0], b[u][0], acc, 0, 0, 0);
       }
+    };
+    int s = wave;
+    for (; s + 8 * (kFewU - 1) < all; s += 8 * kFewU) steps(s, std::integral_constant<int, kFewU>{});
+    if (s + 8 * 3 < all) {
+      steps(s, std::integral_constant<int, 4>{});
+      s += 32;
+    }
+    if (s + 8 < all) {
+      steps(s, std::integral_constant<int, 2>{});
+      s += 16;
+    }
+    if (s < all) steps(s, std::integral_constant<int, 1>{});
   }
+  if (wave > 0) {
+#pragma unroll
+    for (int v = 0; v < 16; v++) part[wave - 1][v * 64 + lane] = acc[v];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int q = 0; q < 7; q++)
+#pragma unroll
+    for (int v = 0; v < 16; v++) acc[v] += part[q][v * 64 + lane];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  floatx16 one[1][1] = {{acc}};
+  ns_epilogue<MODE, 1, 1>(g, one, reinterpret_cast<char*>(part), mat, mw, nw, l32, kh, kSym && tm == tn);
 }
 
 __device__ __forceinline__ float update_of(float g, float m, float mu, int nesterov) {
@@ -324,8 +415,8 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const float* __restrict__ 
 // 1 / (|u|_F + 1e-7) from the partial sums; NaN where the norm is not finite,
 // so that the whole matrix is.
 __device__ __forceinline__ double ns_scale(const double* __restrict__ part, int parts, int* ex = nullptr) {
-  double sq = 0.;
-  for (int p = 0; p < parts; p++) sq += part[p];
+  const int lane = threadIdx.x & 63;  // (parts <= 64)
+  const double sq = wave_sum(lane < parts ? part[lane] : 0.);
   const double norm = sqrt(sq), by = sq < __builtin_inf() ? 1. / (norm + kNsEps) : __builtin_nan("");
   // 2^ex |X0| in (1/2, 1]: |X0| is at least 1e-38, since no smaller float has a square here
   if (ex) *ex = norm * by > 0. ? max(0, min(126, ilogb(1. / (norm * by)))) : 0;
@@ -379,7 +470,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(NsStart a) {
   for (int q = 0; q < 2; q++) {
     const int o = hi + 4 * q;
     half8 h, l;
-    if (i0 + lo < a.M) {
+    if (i0 + lo < a.M && j0 + 8 * o < a.np) {
 #pragma unroll
       for (int u = 0; u < 8; u++) {
         _Float16 hh, ll;
@@ -391,7 +482,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(NsStart a) {
       *reinterpret_cast<half8*>(to) = h;
       *reinterpret_cast<half8*>(to + pg) = l;
     }
-    if (j0 + lo < a.N) {
+    if (j0 + lo < a.N && i0 + 8 * o < a.mp) {
 #pragma unroll
       for (int u = 0; u < 8; u++) {
         _Float16 hh, ll;
@@ -422,6 +513,196 @@ __global__ __launch_bounds__(256) void ns_normalise_kernel(const float* g, const
   }
 }
 
+// A small matrix's whole orthogonalisation by one workgroup of 16 waves: X both
+// ways and S (then P in its place) in LDS as the products above hold them,
+// padded so (8 m N + 4 m^2 bytes: up to 64 x 256).  A step is three products
+// of a few 16 x 16 blocks a wave with a barrier between (blocks of 32 x 32 leave
+// most waves without one).  Bound by the latency of LDS reads and MFMAs.
+constexpr int kNsLds = 163840;
+struct NsFused {
+  const float* g;
+  float* m;
+  float mu;
+  int nesterov, r, c, M, N, mp, np, steps;
+  float* f;
+  float le, decay;
+  int weights;
+};
+__global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
+  extern __shared__ __attribute__((aligned(16))) char ns_lds[];
+  __shared__ double red[16];
+  constexpr int kW = 16, kSymBlocks = 2, kBlocks = 5;  // waves, blocks of S and of X a wave (ns_fused_fits)
+  const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int mp = a.mp, np = a.np, mb = mp / 16, nb = np / 16;
+  _Float16* gram = reinterpret_cast<_Float16*>(ns_lds);  // [2][np / 8][mp][8]
+  _Float16* upd = gram + 2 * np * mp;                    // [2][mp / 8][np][8]
+  _Float16* sym = upd + 2 * np * mp;                     // [2][mp / 8][mp][8]
+  const int px = np * mp, ps = mp * mp;                  // to the other piece
+  const int elems = a.r * a.c;
+  const int64_t base = (int64_t)blockIdx.x * elems;
+  const float* __restrict__ g = a.g + base;
+  float* __restrict__ m = a.m ? a.m + base : nullptr;
+  const bool tall = a.r > a.c;
+  double sq = 0.;
+#pragma unroll 4
+  for (int i = t; i < elems; i += 64 * kW) {
+    float u = g[i];
+    if (m) {
+      const float mm = a.mu * m[i] + u;
+      m[i] = mm;
+      u = update_of(u, mm, a.mu, a.nesterov);
+    }
+    sq += (double)u * u;
+  }
+  sq = wave_sum(sq);
+  if (lane == 0) red[wave] = sq;
+  for (int i = t; i < px / 2; i += 64 * kW) reinterpret_cast<uintx4*>(gram)[i] = uintx4{0u, 0u, 0u, 0u};  // (both of X)
+  __syncthreads();
+  int e0;
+  const double up = ldexp(ns_scale(red, kW, &e0) * kUpX, e0);
+  // a chunk at a time: eight k of a row, of X (i, j) at i * c + j or, tall, j * c + i
+  const int si1 = tall ? 1 : a.c, sj1 = tall ? a.c : 1;
+  auto chunks = [&](_Float16* to, int rows, int nrows, int ks, int row_step, int k_step) {
+    // (rows of the operand in consecutive lanes; octets past the end stay zero)
+    for (int c = t; c < ((ks + 7) >> 3) * nrows; c += 64 * kW) {
+      const int o = c / nrows, row = c - o * nrows;
+      half8 h, l;
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const int k = 8 * o + u;
+        const int at = row * row_step + min(k, ks - 1) * k_step;
+        float v = g[at];
+        if (m) v = update_of(v, m[at], a.mu, a.nesterov);
+        v = k < ks ? (float)(v * up) : 0.f;
+        _Float16 hh, ll;
+        split2(v, hh, ll);
+        h[u] = hh;
+        l[u] = ll;
+      }
+      _Float16* p = to + (o * rows + row) * 8;
+      *reinterpret_cast<half8*>(p) = h;
+      *reinterpret_cast<half8*>(p + px) = l;
+    }
+  };
+  chunks(gram, mp, a.M, a.N, si1, sj1);
+  chunks(upd, np, a.N, a.M, sj1, si1);
+  __syncthreads();
+  // 16 x 16 block (bi, bj) of A B^T over `steps` of 32: lane (l16, kq) holds
+  // octet kq of a step, then column l16 of rows 4 kq ..
+  auto block = [&](const _Float16* A, int ra, int la, int bi, const _Float16* B, int rb, int lb, int bj, int steps) {
+    const half8* pa = reinterpret_cast<const half8*>(A) + kq * ra + bi * 16 + l16;
+    const half8* pb = reinterpret_cast<const half8*>(B) + kq * rb + bj * 16 + l16;
+    la /= 8;
+    lb /= 8;
+    floatx4 hi = {0.f, 0.f, 0.f, 0.f}, lo = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int s = 0; s < steps; s++) {
+      const half8 a0 = pa[4 * s * ra], a1 = pa[4 * s * ra + la], b0 = pb[4 * s * rb], b1 = pb[4 * s * rb + lb];
+      hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b0, hi, 0, 0, 0);
+      lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, b0, lo, 0, 0, 0);
+      lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b1, lo, 0, 0, 0);
+    }
+    return hi + lo;
+  };
+  // a block's values as operand [k = row][col] of rows r and, other not null, as [k = col][row] of rows ro
+  auto put = [&](const floatx4& x, int bi, int bj, _Float16* to, int r, int piece, _Float16* other, int ro) {
+    const int col = bj * 16 + l16, row = bi * 16 + 4 * kq;
+    half4 h, l;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      _Float16 hh, ll;
+      split2(x[u], hh, ll);
+      h[u] = hh;
+      l[u] = ll;
+      if (other) {
+        _Float16* p = other + ((col >> 3) * ro + row + u) * 8 + (col & 7);
+        p[0] = hh;
+        p[piece] = ll;
+      }
+    }
+    _Float16* p = to + ((row >> 3) * r + col) * 8 + (row & 7);
+    *reinterpret_cast<half4*>(p) = h;
+    *reinterpret_cast<half4*>(p + piece) = l;
+  };
+  const int tri = mb * (mb + 1) / 2;
+  int si[kSymBlocks], sj[kSymBlocks];
+#pragma unroll
+  for (int q = 0; q < kSymBlocks; q++) ns_tile<true>(wave + kW * q, 0, si[q], sj[q]);
+  for (int step = 0; step < a.steps; step++) {
+    const int ex = max(0, e0 - 2 * step);
+    floatx4 S[kSymBlocks], P[kSymBlocks];
+#pragma unroll
+    for (int q = 0; q < kSymBlocks; q++) {
+      if (wave + kW * q >= tri) break;
+      S[q] = block(gram, mp, px, si[q], gram, mp, px, sj[q], np / 32);
+#pragma unroll
+      for (int v = 0; v < 4; v++) {
+        // (as P's square sees it: a rounding of S in one term alone would reach P four times as large)
+        _Float16 h, l;
+        split2(S[q][v] * (kUpS / (kUpX * kUpX)), h, l);
+        S[q][v] = (float)h + (float)l;
+      }
+      put(S[q], si[q], sj[q], sym, mp, ps, si[q] == sj[q] ? nullptr : sym, mp);
+    }
+    __syncthreads();
+    const float bs = ldexpf(kNsB * kUpP / kUpS, -2 * ex), bss = ldexpf(kNsC * kUpP / (kUpS * kUpS), -4 * ex);
+#pragma unroll
+    for (int q = 0; q < kSymBlocks; q++) {
+      if (wave + kW * q >= tri) break;
+      P[q] = block(sym, mp, ps, si[q], sym, mp, ps, sj[q], mp / 32);
+      const int col = sj[q] * 16 + l16, row = si[q] * 16 + 4 * kq;
+#pragma unroll
+      for (int v = 0; v < 4; v++)
+        P[q][v] = P[q][v] * bss + (row + v == col && col < a.M ? kNsA * kUpP : 0.f) + bs * S[q][v];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kSymBlocks; q++) {
+      if (wave + kW * q >= tri) break;
+      put(P[q], si[q], sj[q], sym, mp, ps, si[q] == sj[q] ? nullptr : sym, mp);
+    }
+    __syncthreads();
+    floatx4 x[kBlocks];
+#pragma unroll
+    for (int q = 0; q < kBlocks; q++) {
+      const int b = wave + kW * q;
+      if (b >= mb * nb) break;
+      x[q] = block(sym, mp, ps, b / nb, upd, np, px, b % nb, mp / 32);
+    }
+    const bool last = step + 1 == a.steps;
+    const float by = last ? ldexpf(1.f / (kUpX * kUpP), -ex) : ldexpf(1.f / kUpP, max(0, ex - 2) - ex);
+    if (!last) __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kBlocks; q++) {
+      const int b = wave + kW * q;
+      if (b >= mb * nb) break;
+      const int bi = b / nb, bj = b % nb;
+      x[q] *= by;
+      if (!last) {
+        put(x[q], bi, bj, upd, np, px, gram, mp);
+        continue;
+      }
+      const int j = bj * 16 + l16;
+#pragma unroll
+      for (int v = 0; v < 4; v++) {
+        const int i = bi * 16 + 4 * kq + v;
+        if (i >= a.M || j >= a.N) continue;
+        float* p = a.f + base + (tall ? j * a.c + i : i * a.c + j);
+        *p = a.weights ? *p - a.le * x[q][v] - a.decay * *p : x[q][v];
+      }
+    }
+    if (!last) __syncthreads();
+  }
+}
+
+// Whether a matrix fits ns_fused_kernel: its LDS, and its waves' blocks (which the LDS bounds: m is at
+// most 96, 21 blocks of S on 16 waves, and m N at most 20480, 80 blocks of X).
+bool ns_fused_fits(int64_t m, int64_t N) {
+  const int64_t mp = (m + 31) / 32 * 32, np = (N + 31) / 32 * 32;
+  return np <= 4096 && 8 * mp * np + 4 * mp * mp + 128 <= kNsLds;
+}
+
 constexpr int64_t round64(int64_t n) { return (n + 63) / 64 * 64; }
 
 struct NsSizes {
@@ -429,8 +710,8 @@ struct NsSizes {
   NsSizes(int64_t r, int64_t c) {
     m = std::min(r, c);
     N = std::max(r, c);
-    mp = round64(m);
-    np = round64(N);
+    mp = (m + 31) / 32 * 32;
+    np = (N + 31) / 32 * 32;
     gram = 2 * np * m;
     upd = 2 * mp * N;
     sym = 2 * mp * m;
@@ -452,8 +733,8 @@ int launch_product(NsArgs& g, hipStream_t s) {
   else if (tiles(128, 128) >= 256)
     hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 2, 2, 2, 32>), dim3((unsigned)(g.tiles * (int64_t)g.n)), dim3(256), 0, s, g);
   else {
-    tiles(64, 64);
-    hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 2, 1, 1, 64>), dim3((unsigned)(g.tiles * (int64_t)g.n)), dim3(256), 0, s, g);
+    tiles(32, 32);
+    hipLaunchKernelGGL((ns_few_kernel<MODE>), dim3((unsigned)(g.tiles * (int64_t)g.n)), dim3(512), 0, s, g);
   }
   NSH_LAUNCHED();
   return 0;
@@ -483,6 +764,22 @@ int launch_newton_schulz(const float* g, float* q, const MuonNs* step, int64_t n
   float* mom = step ? step->m : nullptr;
   const float mu = step ? step->mu : 0.f;
   const int nesterov = step ? step->nesterov : 0;
+  if (steps > 0 && ns_fused_fits(z.m, z.N)) {
+    NsFused f{};
+    f.g = g; f.m = mom; f.mu = mu; f.nesterov = nesterov;
+    f.r = (int)r; f.c = (int)c; f.M = (int)z.m; f.N = (int)z.N;
+    f.mp = (f.M + 31) / 32 * 32;
+    f.np = (f.N + 31) / 32 * 32;
+    f.steps = steps;
+    f.f = step ? step->w : q;
+    f.weights = step != nullptr;
+    f.le = step ? step->le : 0.f;
+    f.decay = step ? step->decay : 0.f;
+    const unsigned lds = (unsigned)(8 * f.mp * f.np + 4 * f.mp * f.mp);
+    hipLaunchKernelGGL(ns_fused_kernel, dim3((unsigned)n), dim3(1024), lds, s, f);
+    NSH_LAUNCHED();
+    return 0;
+  }
   hipLaunchKernelGGL(ns_norm_kernel, dim3(parts, (unsigned)n), dim3(256), 0, s, g, mom, mu, nesterov, elems, part);
   NSH_LAUNCHED();
   if (steps == 0) {
@@ -498,8 +795,8 @@ int launch_newton_schulz(const float* g, float* q, const MuonNs* step, int64_t n
   a.parts = parts; a.part = part; a.ex = ex;
   a.gram = gram; a.upd = upd;
   a.M = z.m; a.N = z.N; a.mp = z.mp; a.np = z.np;
-  a.tiles_n = (int)(z.np / 64);
-  hipLaunchKernelGGL(ns_start_kernel, dim3((unsigned)(z.mp / 64 * (z.np / 64)), (unsigned)n), dim3(256), 0, s, a);
+  a.tiles_n = (int)ceil_div(z.np, 64);
+  hipLaunchKernelGGL(ns_start_kernel, dim3((unsigned)(ceil_div(z.mp, 64) * a.tiles_n), (unsigned)n), dim3(256), 0, s, a);
   NSH_LAUNCHED();
   for (int k = 0; k < steps; k++) {
     NsArgs p{};
