@@ -372,6 +372,183 @@ __global__ __launch_bounds__(256) void gather_kernel(const float* __restrict__ a
   }
 }
 
+// ---- few slots --------------------------------------------------------------------
+//
+// Where the experts hold a handful of slots each, a product is bound by its
+// weights' bytes, and with one token by latency: no sort, fp32 multiply-adds (8
+// rows cost a quarter of the time that the weights take to arrive).  Workgroup
+// (column tile, expert, K chunk) lists the expert's slots itself and streams 64
+// columns of its chunk once for up to 8 of them (with fewer slots than experts:
+// (column tile, slot, K chunk), and the first of an expert's slots does it); the chunks make enough
+// workgroups to fill the chip and are summed, in their order, by whoever reads
+// them: the second product as it stages act(u), the last pass as it weighs the
+// slots.  64 experts of 1024 x 1024: one token (2 slots) and 37 tokens, us: the
+// sorted products above 186, 197.
+constexpr int kFewSlots = 1024;  // most slots (a list in LDS)
+constexpr int kFewRows = 8;      // rows a pass over the weights
+constexpr int kFewK = 512;       // contraction staged at once
+
+struct FewArgs {
+  const float* in;     // FIRST: x [T, k]; else partial sums [parts][slots, k] of u
+  const float* W;      // [E, k, cols]
+  const int32_t* idx;
+  float* out;          // [chunks][slots, cols]
+  int slots, choices, E, k, cols, chunk, parts, act;
+  bool by_slot;
+};
+
+// Sum of p[0], p[stride], ... in order, four loads in flight.
+__device__ __forceinline__ float sum_parts(const float* __restrict__ p, int64_t stride, int parts) {
+  float v = 0.f;
+  for (int z = 0; z < parts; z += 4) {
+    float x[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) x[u] = p[min(z + u, parts - 1) * stride];
+#pragma unroll
+    for (int u = 0; u < 4; u++) v += z + u < parts ? x[u] : 0.f;
+  }
+  return v;
+}
+
+// VEC: 16 lanes of four columns and four k a wave, else 64 columns.
+template <bool FIRST, int VEC>
+__global__ __launch_bounds__(256) void few_kernel(FewArgs a) {
+  constexpr int KR = VEC == 4 ? 4 : 1, STEP = 4 * KR, UN = 8;
+  __shared__ int list[kFewSlots];
+  __shared__ int count;
+  __shared__ __attribute__((aligned(16))) float xs[kFewK * kFewRows];
+  __shared__ float red[4][kFewRows * 64];
+  const int t = threadIdx.x, lane = t & 63;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int e = a.by_slot ? a.idx[blockIdx.y] : (int)blockIdx.y;
+  if (e < 0 || e >= a.E) return;
+  if (w == 0) {
+    int n = 0;
+    for (int s = lane; s < a.slots + lane; s += 64) {
+      const uint64_t m = __ballot(s < a.slots && a.idx[s < a.slots ? s : 0] == e);
+      if ((m >> lane) & 1) list[n + __builtin_popcountll(m & ((1ull << lane) - 1))] = s;
+      n += __builtin_popcountll(m);
+    }
+    if (lane == 0) count = n;
+  }
+  __syncthreads();
+  const int n = count;
+  if (n == 0 || (a.by_slot && list[0] != (int)blockIdx.y)) return;
+  const int kbeg = blockIdx.z * a.chunk, kend = min(a.k, kbeg + a.chunk);
+  const int lc = VEC == 4 ? (lane & 15) * 4 : lane, kr = VEC == 4 ? lane >> 4 : 0;
+  const int col0 = blockIdx.x * 64;
+  const int col = min(col0 + lc, a.cols - VEC);  // (columns past the end are not stored)
+  const float* __restrict__ W = a.W + (int64_t)e * a.k * a.cols + col;
+  float* __restrict__ out = a.out + (int64_t)blockIdx.z * a.slots * a.cols;
+  auto pass = [&](int r0, auto rows) {
+    constexpr int R = decltype(rows)::value;
+    const int nr = min(R, n - r0);
+    float acc[R][VEC];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int j = 0; j < VEC; j++) acc[r][j] = 0.f;
+    for (int k0 = kbeg; k0 < kend; k0 += kFewK) {
+      const int kn = min(kFewK, kend - k0);
+      __syncthreads();  // (the last stage is read)
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const int slot = list[r0 + min(r, nr - 1)];
+        for (int k = t; k < kn; k += 256) {
+          float v;
+          if (FIRST) {
+            v = a.in[(int64_t)(slot / a.choices) * a.k + k0 + k];
+          } else {
+            const float* p = a.in + (int64_t)slot * a.k + k0 + k;
+            v = sum_parts(p, (int64_t)a.slots * a.k, a.parts);
+            v = act_apply(v, a.act);
+          }
+          xs[k * R + r] = r < nr ? v : 0.f;
+        }
+      }
+      __syncthreads();
+      auto steps = [&](int kk, auto count, auto check) {
+        constexpr int CNT = decltype(count)::value;
+        constexpr bool CHK = decltype(check)::value;
+        float v[CNT][VEC];
+#pragma unroll
+        for (int u = 0; u < CNT; u++) {
+          const int k = kk + u * STEP;
+          const float* q = W + (int64_t)(k0 + (CHK ? min(k, kn - 1) : k)) * a.cols;
+          if (VEC == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(q);
+            v[u][0] = f.x; v[u][VEC / 4] = f.y; v[u][VEC / 2] = f.z; v[u][VEC - 1] = f.w;
+          } else {
+            v[u][0] = *q;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < CNT; u++) {
+          const int k = kk + u * STEP;
+          const float* x = xs + (CHK ? min(k, kn - 1) : k) * R;
+#pragma unroll
+          for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+              const float f = CHK && k >= kn ? 0.f : v[u][j];
+              acc[r][j] = fmaf(CHK && k >= kn ? 0.f : x[r], f, acc[r][j]);
+            }
+        }
+      };
+      int kk = w * KR + kr, left = kn;
+      for (; left >= UN * STEP; left -= UN * STEP, kk += UN * STEP)
+        steps(kk, std::integral_constant<int, UN>{}, std::false_type{});
+      for (; left > 0; left -= 2 * STEP, kk += 2 * STEP) steps(kk, std::integral_constant<int, 2>{}, std::true_type{});
+    }
+    if (VEC == 4) {
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+          acc[r][j] += __shfl_xor(acc[r][j], 16, kWave);
+          acc[r][j] += __shfl_xor(acc[r][j], 32, kWave);
+        }
+    }
+    if (VEC == 1 || lane < 16) {
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < VEC; j++) red[w][r * 64 + lc + j] = acc[r][j];
+    }
+    __syncthreads();
+    for (int i = t; i < nr * 64; i += 256) {
+      const int c = col0 + (i & 63);
+      if (c < a.cols)
+        out[(int64_t)list[r0 + (i >> 6)] * a.cols + c] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+    }
+  };
+  for (int r0 = 0; r0 < n; r0 += kFewRows) {
+    const int left = n - r0;
+    if (left == 1) pass(r0, std::integral_constant<int, 1>{});
+    else if (left == 2) pass(r0, std::integral_constant<int, 2>{});
+    else if (left <= 4) pass(r0, std::integral_constant<int, 4>{});
+    else pass(r0, std::integral_constant<int, 8>{});
+    __syncthreads();  // (red is read)
+  }
+}
+
+// y[t] = sum over the token's slots of weight * (sum over the chunks of o)
+__global__ __launch_bounds__(256) void few_combine_kernel(const float* __restrict__ o, const int32_t* __restrict__ idx,
+                                                          const float* __restrict__ weight, float* __restrict__ y,
+                                                          int64_t n, int choices, int cols, int E, int slots,
+                                                          int parts) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int t = (int)(i / cols), c = (int)(i - (int64_t)t * cols);
+  float y0 = 0.f;
+  for (int k = 0; k < choices; k++) {
+    const int slot = t * choices + k, e = idx[slot];
+    if (e < 0 || e >= E) continue;
+    y0 += weight[slot] * sum_parts(o + (int64_t)slot * cols + c, (int64_t)slots * cols, parts);
+  }
+  y[i] = y0;
+}
+
 struct Tables {
   int *seg, *perm, *tok, *expert, *tiles, *ntiles;
 };
@@ -452,6 +629,52 @@ int launch_route_grad(const RouteGradArgs& a, hipStream_t s) {
   return 0;
 }
 
+// Whether the layer runs without a sort: up to 6 slots an expert on average.  64
+// experts of 1024 x 1024, two slots a token, us, this and sorted: 1 token 12,
+// 186; 32 tokens 87, 198; 128 137, 204; 200 184, 207; 256 217, 208.
+constexpr int kFewPerExpert = 6;
+static bool few_slots(const MoeShape& m) { return m.T * m.K <= kFewSlots && m.T * m.K <= kFewPerExpert * m.E; }
+// K chunks of a product [.., k] x [k, cols] over the experts that `slots` reach:
+// about 256 workgroups, of 64 steps of K at least (64 experts of 1024 x 1024, 1
+// and 8 tokens of 2 slots, us: 128 workgroups 11.1, 33.3; 256 11.6, 33.3; 512
+// 15.3, 27.5; 1024 15.2, 30.1: the chunks' sums cost a round trip for each four).
+static int few_chunks(int64_t k, int64_t cols, int64_t slots, int64_t E) {
+  const int64_t wgs = ceil_div(cols, 64) * std::min(slots, E);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, ceil_div(256, wgs)), k / 64));
+}
+
+static int launch_few(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2,
+                      float* y, const MoeShape& m, int act, void* workspace, hipStream_t s) {
+  const int64_t N = m.T * m.K;
+  FewArgs a;
+  a.slots = (int)N; a.choices = (int)m.K; a.E = (int)m.E; a.idx = idx; a.act = act;
+  a.by_slot = N < m.E;
+  auto product = [&](auto first, int64_t k, int64_t cols, const float* W) {
+    constexpr bool FIRST = decltype(first)::value;
+    const int chunks = few_chunks(k, cols, N, m.E);
+    a.W = W; a.k = (int)k; a.cols = (int)cols;
+    a.chunk = (int)ceil_div(k, chunks);
+    const dim3 g((unsigned)ceil_div(cols, 64), (unsigned)std::min(N, m.E), (unsigned)ceil_div(k, a.chunk));
+    if (cols % 4 == 0 && (reinterpret_cast<uintptr_t>(W) & 15) == 0)
+      hipLaunchKernelGGL((few_kernel<FIRST, 4>), g, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((few_kernel<FIRST, 1>), g, dim3(256), 0, s, a);
+    return (int)g.z;
+  };
+  float* u = static_cast<float*>(workspace);
+  float* o = u + round64(few_chunks(m.D, m.H, N, m.E) * N * m.H);
+  a.in = x; a.out = u; a.parts = 1;
+  a.parts = product(std::true_type{}, m.D, m.H, W1);
+  NSH_LAUNCHED();
+  a.in = u; a.out = o;
+  const int parts = product(std::false_type{}, m.H, m.D, W2);
+  NSH_LAUNCHED();
+  hipLaunchKernelGGL(few_combine_kernel, dim3((unsigned)ceil_div(m.T * m.D, 256)), dim3(256), 0, s, o, idx, weight, y,
+                     m.T * m.D, (int)m.K, (int)m.D, (int)m.E, (int)N, parts);
+  NSH_LAUNCHED();
+  return 0;
+}
+
 // state: the sorted slots' tables, then the pre-activations [T K, H]
 size_t experts_state_bytes(const MoeShape& m) {
   const int64_t N = m.T * m.K;
@@ -464,13 +687,17 @@ size_t experts_workspace_bytes(const MoeShape& m, bool grad) {
   const int64_t N = m.T * m.K;
   const int64_t fwd = count_ints(N, m.E) + tables_ints(N, m.E) + round64(N * m.H) + N * m.D;
   const int64_t bwd = 2 * round64(N * m.H) + 3 * round64(N * m.D);
-  return 4 * (size_t)std::max(fwd, grad ? bwd : 0);
+  const int64_t few = few_slots(m) ? round64(few_chunks(m.D, m.H, N, m.E) * N * m.H) +
+                                         few_chunks(m.H, m.D, N, m.E) * N * m.D
+                                   : 0;
+  return 4 * (size_t)std::max(std::max(fwd, few), grad ? bwd : 0);
 }
 
 int launch_experts(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2, float* y,
                    const MoeShape& m, int act, void* state, void* workspace, hipStream_t s) {
   const int64_t N = m.T * m.K;
   if (m.T <= 0 || m.D <= 0) return 0;
+  if (!state && few_slots(m)) return launch_few(x, idx, weight, W1, W2, y, m, act, workspace, s);
   int* wi = static_cast<int*>(workspace);
   int* count = wi;
   wi += count_ints(N, m.E);
