@@ -685,7 +685,8 @@ struct Bf3Stage {
 
 // The activations that the split kernel's epilogues hold, by use: a dense
 // layer's (NN) all; transposed products (gradients) and the general epilogue
-// none; an expert layer's GELU.  bf3_takes sends the rest elsewhere.
+// none; a grouped layer's all, in an instantiation beside that of the top-1
+// expert layer's GELU.  bf3_takes sends the rest elsewhere.
 constexpr unsigned kActsNone = 1u << kActId;
 constexpr unsigned kActsMoe = 1u << kActId | 1u << kActGeluMoe;
 
@@ -1020,7 +1021,7 @@ constexpr int kBf3MinK = 128;
 static bool bf3_takes(const GemmArgs& g, bool vec, bool plain, bool tA, bool tB) {
   if (!vec || (tA && tB) || g.f32 || g.K < kBf3MinK) return false;
   if (g.mode == kEpiAccum || (plain && g.mode == kEpiActGrad)) return true;
-  const unsigned acts = !plain || tA || tB ? kActsNone : g.groups ? kActsMoe : kAllActs;
+  const unsigned acts = !plain || tA || tB ? kActsNone : kAllActs;
   return g.mode == kEpiAct && ((acts >> g.act) & 1);
 }
 
@@ -1143,7 +1144,7 @@ int launch_gemm_ex(const GemmArgs& in, bool tA, bool tB, int batch, hipStream_t 
   const bool bf3 = bf3_takes(g, vec, plain, tA, tB);
   int bm = BM, bn = BN, tile = kT128;
   if (bf3 && g.groups) {
-    bn = 256;  // 128-row tiles (the caller's tile list), 256 columns
+    bn = g.narrow ? 128 : 256;  // 128-row tiles (the caller's tile list), 256 columns
   } else if (bf3 && plain && !g.kitems && !g.kseg) {
     tile = pick_tile(g, true, batch, zs, zs, cus).tile;
     bm = tile == kT128 ? 128 : 256;
@@ -1166,8 +1167,15 @@ int launch_gemm_ex(const GemmArgs& in, bool tA, bool tB, int batch, hipStream_t 
       hipLaunchKernelGGL((gemm_bf3_kernel<TA_, TB_, true, ACTS_, 4, 2>), grid, dim3(512), 0, s, g);             \
     else hipLaunchKernelGGL((gemm_bf3_kernel<TA_, TB_, true, ACTS_, 2, 2>), grid, dim3(256), 0, s, g);          \
   } while (0)
-  if (bf3 && g.groups) {
-    if (!tB && plain) hipLaunchKernelGGL((gemm_bf3_kernel<false, false, true, kActsMoe, 2, 4>), grid, dim3(512), 0, s, g);
+  if (bf3 && g.groups && g.narrow) {
+    if (!tB && plain) hipLaunchKernelGGL((gemm_bf3_kernel<false, false, true, kAllActs, 2, 2>), grid, dim3(256), 0, s, g);
+    else if (!tB) hipLaunchKernelGGL((gemm_bf3_kernel<false, false, false, kActsNone, 2, 2>), grid, dim3(256), 0, s, g);
+    else if (plain) hipLaunchKernelGGL((gemm_bf3_kernel<false, true, true, kActsNone, 2, 2>), grid, dim3(256), 0, s, g);
+    else hipLaunchKernelGGL((gemm_bf3_kernel<false, true, false, kActsNone, 2, 2>), grid, dim3(256), 0, s, g);
+  } else if (bf3 && g.groups) {
+    if (!tB && plain && ((kActsMoe >> g.act) & 1))
+      hipLaunchKernelGGL((gemm_bf3_kernel<false, false, true, kActsMoe, 2, 4>), grid, dim3(512), 0, s, g);
+    else if (!tB && plain) hipLaunchKernelGGL((gemm_bf3_kernel<false, false, true, kAllActs, 2, 4>), grid, dim3(512), 0, s, g);
     else if (!tB) hipLaunchKernelGGL((gemm_bf3_kernel<false, false, false, kActsNone, 2, 4>), grid, dim3(512), 0, s, g);
     else if (plain) hipLaunchKernelGGL((gemm_bf3_kernel<false, true, true, kActsNone, 2, 4>), grid, dim3(512), 0, s, g);
     else hipLaunchKernelGGL((gemm_bf3_kernel<false, true, false, kActsNone, 2, 4>), grid, dim3(512), 0, s, g);

@@ -74,6 +74,8 @@ struct GemmArgs {
   // separately stored products, e.g. dX = [dQ dK dV] . [Wq Wk Wv]^T.
   int kblk = 0;
   int64_t sAk = 0, sBk = 0;
+  // grouped mode: 128 columns a tile instead of 256
+  bool narrow = false;
   // fp32 MFMA only (a top-1 router's gradients: moe.hip)
   bool f32 = false;
   int tiles_m = 0, tiles_n = 0;    // filled by the launcher
@@ -238,6 +240,13 @@ size_t moe_bwd_kpart_floats(int64_t M, int64_t D, int64_t H);
 // Floats of MoeBwdWork::splitk that let dWg = x^T dg (K = M tokens, only
 // D x E outputs) run split over K; 0 when it would not be split.
 size_t moe_bwd_splitk_floats(int64_t M, int64_t D, int64_t E);
+// The work items over the segments seg [E + 1] of M sorted rows (dirty: as
+// MoeBwdWork::dirty, or null), and a weight gradient C[e] [R, Cc] = A[seg e]^T
+// B[seg e] over them (R, Cc: D, H or H, D; A [M, R], B [M, Cc]).
+int launch_moe_kitems(const int* seg, int* kitems, int* dirty, int64_t M, int64_t D, int64_t H, int64_t E,
+                      hipStream_t s);
+int launch_moe_weight_grad(const float* A, const float* B, float* C, int64_t R, int64_t Cc, const int* kitems,
+                           float* kpart, int64_t M, int64_t D, int64_t H, int64_t E, hipStream_t s);
 size_t moe_work_ints(int64_t M, int64_t E);   // int-sized words of all int arrays
 int launch_moe_route(const float* x, const float* Wg, const uint8_t* active, const MoeWork& w, int64_t M, int64_t D,
                      int64_t E, hipStream_t s);

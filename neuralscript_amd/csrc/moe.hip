@@ -918,6 +918,39 @@ __global__ __launch_bounds__(256) void moe_kpart_sum_kernel(const int* __restric
   }
 }
 
+int launch_moe_kitems(const int* seg, int* kitems, int* dirty, int64_t M, int64_t D, int64_t H, int64_t E,
+                      hipStream_t s) {
+  hipLaunchKernelGGL(moe_kitems_kernel, dim3(1), dim3(256), 0, s, seg, (int)E, (int)kchunk_of(M, D, H),
+                     (int)kitems_max(M, D, H, E), kitems, dirty);
+  NSH_LAUNCHED();
+  return 0;
+}
+
+int launch_moe_weight_grad(const float* A, const float* B, float* C, int64_t R, int64_t Cc, const int* kitems,
+                           float* kpart, int64_t M, int64_t D, int64_t H, int64_t E, hipStream_t s) {
+  const int maxitems = (int)kitems_max(M, D, H, E), maxred = (int)kreduce_max(M, D, H);
+  GemmArgs k;
+  k.A = A; k.B = B; k.C = C;
+  k.M = (int)R; k.N = (int)Cc; k.K = (int)M;
+  k.lda = R; k.ldb = Cc; k.ldc = Cc;
+  k.sC = R * Cc;
+  k.kitems = kitems + 2; k.nkitems = kitems; k.kpart = kpart;
+  if (launch_gemm_ex(k, true, false, maxitems, s) != 0) return -1;
+  if (maxred > 0) {
+    const int64_t DH = R * Cc;
+    const bool vec = DH % 4 == 0 && ((reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(kpart)) & 15) == 0;
+    // one element (float4) per thread: each entry's sum is a few MB, and
+    // fewer threads looping over it left the pass latency-bound
+    const unsigned gx = (unsigned)std::min<int64_t>(ceil_div(vec ? DH / 4 : DH, 256), 4096);
+    if (vec)
+      hipLaunchKernelGGL(moe_kpart_sum_kernel<true>, dim3(gx, maxred), dim3(256), 0, s, kitems, maxitems, kpart, C, DH);
+    else
+      hipLaunchKernelGGL(moe_kpart_sum_kernel<false>, dim3(gx, maxred), dim3(256), 0, s, kitems, maxitems, kpart, C, DH);
+    NSH_LAUNCHED();
+  }
+  return 0;
+}
+
 // dWg[D, E] = x[M, D]^T dg[M, E]
 static GemmArgs dwg_args(const float* x, const float* dg, float* dWg, int64_t M, int64_t D, int64_t E) {
   GemmArgs g;
@@ -1009,39 +1042,16 @@ int launch_moe_backward(const float* x, const float* dout, const float* Wg, cons
   // token chunks of each expert (without the work buffers: one K range per
   // expert)
   const bool chunked = b.kitems && (b.kpart || kreduce_max(M, D, H) == 0);
-  const int maxitems = (int)kitems_max(M, D, H, E), maxred = (int)kreduce_max(M, D, H);
-  if (chunked) {
-    hipLaunchKernelGGL(moe_kitems_kernel, dim3(1), dim3(256), 0, s, w.seg, (int)E, (int)kchunk_of(M, D, H), maxitems,
-                       b.kitems, b.dirty);
-    NSH_LAUNCHED();
-  }
+  if (chunked && launch_moe_kitems(w.seg, b.kitems, b.dirty, M, D, H, E, s) != 0) return -1;
   auto weight_grad = [&](const float* A, const float* B, float* C, int64_t R, int64_t Cc) -> int {
+    if (chunked) return launch_moe_weight_grad(A, B, C, R, Cc, b.kitems, b.kpart, M, D, H, E, s);
     GemmArgs k;
     k.A = A; k.B = B; k.C = C;
     k.M = (int)R; k.N = (int)Cc; k.K = (int)M;
     k.lda = R; k.ldb = Cc; k.ldc = Cc;
     k.sC = R * Cc;
-    if (!chunked) {
-      k.kseg = w.seg;
-      return launch_gemm_ex(k, true, false, (int)E, s);
-    }
-    k.kitems = b.kitems + 2; k.nkitems = b.kitems; k.kpart = b.kpart;
-    if (launch_gemm_ex(k, true, false, maxitems, s) != 0) return -1;
-    if (maxred > 0) {
-      const int64_t DH = R * Cc;
-      const bool vec = DH % 4 == 0 && ((reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(b.kpart)) & 15) == 0;
-      // one element (float4) per thread: each entry's sum is a few MB, and
-      // fewer threads looping over it left the pass latency-bound
-      const unsigned gx = (unsigned)std::min<int64_t>(ceil_div(vec ? DH / 4 : DH, 256), 4096);
-      if (vec)
-        hipLaunchKernelGGL(moe_kpart_sum_kernel<true>, dim3(gx, maxred), dim3(256), 0, s, b.kitems, maxitems, b.kpart,
-                           C, DH);
-      else
-        hipLaunchKernelGGL(moe_kpart_sum_kernel<false>, dim3(gx, maxred), dim3(256), 0, s, b.kitems, maxitems, b.kpart,
-                           C, DH);
-      NSH_LAUNCHED();
-    }
-    return 0;
+    k.kseg = w.seg;
+    return launch_gemm_ex(k, true, false, (int)E, s);
   };
   // dWe1[e] [D, H] = xs[seg e]^T dH[seg e]
   if (dWe1 && weight_grad(b.xs, b.dH, dWe1, D, H) != 0) return -1;

@@ -300,14 +300,6 @@ __global__ __launch_bounds__(kSortBlock) void slots_place_kernel(const int32_t* 
 
 // ---- rows ---------------------------------------------------------------------------
 
-// h = act(u) over the rows [0, *nrows) of H
-__global__ __launch_bounds__(256) void act_rows_kernel(const float* __restrict__ u, float* __restrict__ h,
-                                                       const int* __restrict__ nrows, int64_t H, int act) {
-  const int64_t n = (int64_t)*nrows * H;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-    h[i] = act_apply(u[i], act);
-}
-
 // y[t] = sum over the token's slots, in order, of o[slot]; slots without an
 // expert add nothing (their rows of o are not written).
 template <int W>
@@ -600,6 +592,7 @@ GemmArgs grouped(const Tables& t, int64_t rows, int64_t N, int64_t K, const floa
   g.M = (int)rows; g.N = (int)N; g.K = (int)K;
   g.lda = K; g.ldb = tB ? K : N; g.ldc = N;
   g.groups = (int)m.E; g.seg = t.seg; g.tiles = t.tiles; g.ntiles = t.ntiles; g.sBg = N * K;
+  g.narrow = N <= 128;
   return g;
 }
 
@@ -682,11 +675,12 @@ size_t experts_state_bytes(const MoeShape& m) {
 }
 // workspace: the sort's counts, the tables (no state), then of the forward
 // hidden [N, H] and slots [N, D]; of the backward dh, hw [N, H], x and dy
-// sorted and the slots [N, D]
+// sorted and the slots [N, D], and the weight gradients' items and partial sums
 size_t experts_workspace_bytes(const MoeShape& m, bool grad) {
   const int64_t N = m.T * m.K;
   const int64_t fwd = count_ints(N, m.E) + tables_ints(N, m.E) + round64(N * m.H) + N * m.D;
-  const int64_t bwd = 2 * round64(N * m.H) + 3 * round64(N * m.D);
+  const int64_t bwd = 2 * round64(N * m.H) + 3 * round64(N * m.D) + round64(moe_bwd_kpart_floats(N, m.D, m.H)) +
+                      moe_bwd_kitem_ints(N, m.D, m.H, m.E);
   const int64_t few = few_slots(m) ? round64(few_chunks(m.D, m.H, N, m.E) * N * m.H) +
                                          few_chunks(m.H, m.D, N, m.E) * N * m.D
                                    : 0;
@@ -706,14 +700,15 @@ int launch_experts(const float* x, const int32_t* idx, const float* weight, cons
   float* hidden = reinterpret_cast<float*>(wi);
   float* slots = hidden + round64(N * m.H);
   const Tables t = tables_at(ti, N, m.E);
-  float* pre = hidden;
-  if (state) pre = reinterpret_cast<float*>(ti + tables_ints(N, m.E));
   if (sort_slots(idx, t, count, N, (int)m.K, (int)m.E, s) != 0) return -1;
-  GemmArgs g = grouped(t, N, m.H, m.D, x, W1, pre, m, false);
+  GemmArgs g = grouped(t, N, m.H, m.D, x, W1, hidden, m, false);
   g.a_rows = t.tok;
+  g.act = act;
+  if (state) {  // the pre-activation stays for the gradient
+    g.C = reinterpret_cast<float*>(ti + tables_ints(N, m.E));
+    g.C2 = hidden;
+  }
   if (launch_gemm_ex(g, false, false, 1, s) != 0) return -1;
-  hipLaunchKernelGGL(act_rows_kernel, dim3(stream_blocks(N * m.H)), dim3(256), 0, s, pre, hidden, t.seg + m.E, m.H, act);
-  NSH_LAUNCHED();
   GemmArgs g2 = grouped(t, N, m.D, m.H, hidden, W2, slots, m, false);
   g2.c_rows = t.perm;
   g2.row_scale = weight;
@@ -738,6 +733,8 @@ int launch_experts_grad(const float* dy, const float* x, const float* weight, co
   float* xs = hw + round64(N * m.H);
   float* dys = xs + round64(N * m.D);
   float* slots = dys + round64(N * m.D);
+  float* kpart = slots + round64(N * m.D);
+  int* kitems = reinterpret_cast<int*>(kpart + round64(moe_bwd_kpart_floats(N, m.D, m.H)));
   const int* nrows = t.seg + m.E;
   GemmArgs g = grouped(t, N, m.H, m.D, dy, W2, dh, m, true);
   g.a_rows = t.tok;
@@ -755,17 +752,9 @@ int launch_experts_grad(const float* dy, const float* x, const float* weight, co
   if (!dW1 && !dW2) return 0;
   hipLaunchKernelGGL(gather_kernel, dim3(stream_blocks(N * m.D)), dim3(256), 0, s, x, dy, t.tok, nrows, xs, dys, m.D);
   NSH_LAUNCHED();
-  auto weight_grad = [&](const float* A, const float* B, float* C, int64_t R, int64_t Cc) {
-    GemmArgs k;
-    k.A = A; k.B = B; k.C = C;
-    k.M = (int)R; k.N = (int)Cc; k.K = (int)N;
-    k.lda = R; k.ldb = Cc; k.ldc = Cc;
-    k.sC = R * Cc;
-    k.kseg = t.seg;
-    return launch_gemm_ex(k, true, false, (int)m.E, s);
-  };
-  if (dW1 && weight_grad(xs, dh, dW1, m.D, m.H) != 0) return -1;
-  if (dW2 && weight_grad(hw, dys, dW2, m.H, m.D) != 0) return -1;
+  if (launch_moe_kitems(t.seg, kitems, nullptr, N, m.D, m.H, m.E, s) != 0) return -1;
+  if (dW1 && launch_moe_weight_grad(xs, dh, dW1, m.D, m.H, kitems, kpart, N, m.D, m.H, m.E, s) != 0) return -1;
+  if (dW2 && launch_moe_weight_grad(hw, dys, dW2, m.H, m.D, kitems, kpart, N, m.D, m.H, m.E, s) != 0) return -1;
   return 0;
 }
 
