@@ -203,6 +203,265 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
   }
 }
 
+// ---- up to 256 experts, up to 16 choices: 16 lanes a token ----
+//
+// Four tokens a wave: a row of 16 lanes holds a token's experts, V consecutive
+// ones a lane, and reduces over itself by DPP moves alone (a whole wave's
+// butterfly goes through LDS: six round trips a choice).  Bound by the 64-bit
+// arithmetic: 16384 tokens of 256 experts, 8 groups, 8 choices: see launch_route.
+template <int CTRL>
+__device__ __forceinline__ int dpp_int(int v) {
+  return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, true);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)dpp_int<CTRL>((int)(uint32_t)b), hi = (uint32_t)dpp_int<CTRL>((int)(uint32_t)(b >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror, row_mirror: after each, all
+// of 2, 4, 8, 16 lanes hold the same.
+template <int CTRL>
+__device__ __forceinline__ void best_step(double& v, int& i) {
+  const double w = dpp_f64<CTRL>(v);
+  const int j = dpp_int<CTRL>(i);
+  const bool take = (int)(w > v) | ((int)(w == v) & (int)(j < i));
+  v = take ? w : v;
+  i = take ? j : i;
+}
+__device__ __forceinline__ void row_best(double& v, int& i) {
+  best_step<0xB1>(v, i);
+  best_step<0x4E>(v, i);
+  best_step<0x141>(v, i);
+  best_step<0x140>(v, i);
+}
+__device__ __forceinline__ double row_sum_f64(double v) {
+  v += dpp_f64<0xB1>(v);
+  v += dpp_f64<0x4E>(v);
+  v += dpp_f64<0x141>(v);
+  return v + dpp_f64<0x140>(v);
+}
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, dpp_mov<0xB1>(v));
+  v = fmaxf(v, dpp_mov<0x4E>(v));
+  v = fmaxf(v, dpp_mov<0x141>(v));
+  return fmaxf(v, dpp_mov<0x140>(v));
+}
+
+// Logits of V consecutive experts from e0, -inf where not live (see live_logit).
+template <int V, bool VEC>
+__device__ __forceinline__ void live_logits(const float* __restrict__ l, int e0, int E,
+                                            const uint8_t* __restrict__ active, float (&x)[V]) {
+  if constexpr (VEC) {  // (E % 4 == 0: a float4 is whole or out)
+#pragma unroll
+    for (int v = 0; v < V; v += 4) {
+      const bool in = e0 + v < E;
+      const float4 f = *reinterpret_cast<const float4*>(l + (in ? e0 + v : 0));
+      const float y[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int on = active ? active[in ? e0 + v + j : 0] : 1;
+        x[v + j] = (int)in & (int)(on != 0) & (int)(y[j] > -__builtin_inff()) ? y[j] : -__builtin_inff();
+      }
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; v++) x[v] = live_logit(l, e0 + v, E, active);
+  }
+}
+
+template <int V, bool VEC>
+__global__ __launch_bounds__(256) void route_row_kernel(RouteArgs a) {
+  __shared__ double by_expert[16][16 * V + 1];
+  const int lane = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const int64_t at = (int64_t)blockIdx.x * 16 + row;
+  const bool in = at < a.T;
+  const int64_t tok = in ? at : a.T - 1;  // (the rows past the end repeat the last token and store nothing)
+  const int e0 = lane * V;
+  float x[V], mx = -__builtin_inff();
+  live_logits<V, VEC>(a.logits + tok * a.E, e0, a.E, a.active, x);
+#pragma unroll
+  for (int v = 0; v < V; v++) mx = fmaxf(mx, x[v]);
+  mx = row_max(mx);
+  double s[V], c[V], softmax_by = 0.;
+  if (a.score == 0) {
+    double sum = 0.;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const double z = x[v] == mx ? 0. : (double)x[v] - (double)mx;  // (a logit of +inf: 0)
+      s[v] = x[v] > -__builtin_inff() ? exp(z) : 0.;
+      sum += s[v];
+    }
+    sum = row_sum_f64(sum);
+    softmax_by = sum > 0. ? 1. / sum : 0.;
+#pragma unroll
+    for (int v = 0; v < V; v++) s[v] *= softmax_by;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; v++) s[v] = x[v] > -__builtin_inff() ? 1. / (1. + exp(-(double)x[v])) : 0.;
+  }
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const double b = s[v] + (a.bias ? (double)a.bias[min(e0 + v, a.E - 1)] : 0.);
+    c[v] = (int)(x[v] > -__builtin_inff()) & (int)(b > kNone) ? b : kNone;
+  }
+  if (a.groups > 1) {
+    const int per = a.E / a.groups;
+    uint64_t keep = 0;
+    double one = kNone, two = kNone;
+    auto merge = [&](double b) {
+      two = b > one ? one : b > two ? b : two;
+      one = b > one ? b : one;
+    };
+    if (per % V == 0) {  // (uniform) a lane's experts lie in one group, a group is `lanes` lanes
+      const int lanes = per / V, g = lane / lanes, base = (threadIdx.x & 48) + g * lanes;
+#pragma unroll
+      for (int v = 0; v < V; v++) merge(c[v]);
+      const double mine1 = one, mine2 = two;
+      for (int o = 1; o < lanes; o++) {
+        int from = lane - g * lanes + o;
+        from = base + (from >= lanes ? from - lanes : from);
+        const double b1 = __shfl(mine1, from, kWave), b2 = __shfl(mine2, from, kWave);
+        merge(b1);
+        merge(b2);
+      }
+      double value = (int)(a.group_best == 2) & (int)(two > kNone) ? one + two : one;
+      value = g < a.groups ? value : kNone;
+      for (int j = 0; j < a.top_groups; j++) {
+        double v = value;
+        int i = g;
+        row_best(v, i);
+        keep |= v > kNone ? 1ull << i : 0;
+        value = i == g ? kNone : value;
+      }
+    } else {
+      double* __restrict__ t = by_expert[row];
+#pragma unroll
+      for (int v = 0; v < V; v++) t[e0 + v] = c[v];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      double value[4];  // groups lane, lane + 16, ..
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const int g = lane + 16 * q;
+        one = two = kNone;
+        if (g < a.groups)
+          for (int j = 0; j < per; j++) merge(t[g * per + j]);
+        value[q] = (int)(a.group_best == 2) & (int)(two > kNone) ? one + two : one;
+      }
+      for (int j = 0; j < a.top_groups; j++) {
+        double v = value[0];
+        int i = lane;
+#pragma unroll
+        for (int q = 1; q < 4; q++) {
+          const bool more = value[q] > v;
+          v = more ? value[q] : v;
+          i = more ? lane + 16 * q : i;
+        }
+        row_best(v, i);
+        keep |= v > kNone ? 1ull << i : 0;
+#pragma unroll
+        for (int q = 0; q < 4; q++) value[q] = i == lane + 16 * q ? kNone : value[q];
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; v++) c[v] = (keep >> (min(e0 + v, a.E - 1) / per)) & 1 ? c[v] : kNone;
+  }
+  int mine = -1;
+  for (int k = 0; k < a.K; k++) {
+    double v = c[0];
+    int i = e0;
+#pragma unroll
+    for (int u = 1; u < V; u++) {
+      const bool more = c[u] > v;
+      v = more ? c[u] : v;
+      i = more ? e0 + u : i;
+    }
+    row_best(v, i);
+    const bool some = v > kNone;
+#pragma unroll
+    for (int u = 0; u < V; u++) c[u] = i == e0 + u ? kNone : c[u];
+    mine = (int)some & (int)(lane == k) ? i : mine;
+  }
+  // the score of this lane's choice, once more
+  double ms = 0.;
+  if (mine >= 0) {
+    const float xm = a.logits[tok * a.E + mine];
+    ms = a.score ? 1. / (1. + exp(-(double)xm)) : (xm == mx ? 1. : exp((double)xm - (double)mx)) * softmax_by;
+  }
+  const double by = a.renorm ? row_sum_f64(ms) : 1.;
+  if (in && lane < a.K) {
+    a.idx[tok * a.K + lane] = mine;
+    a.weight[tok * a.K + lane] = by > 0. ? (float)((double)a.scale * ms / by) : 0.f;
+  }
+}
+
+template <int V, bool VEC>
+__global__ __launch_bounds__(256) void route_grad_row_kernel(RouteGradArgs a) {
+  const int lane = threadIdx.x & 15;
+  const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const bool in = at < a.T;
+  const int64_t tok = in ? at : a.T - 1;
+  const float* __restrict__ l = a.logits + tok * a.E;
+  const int e0 = lane * V;
+  // this lane's choice
+  int mine = -1;
+  float dw = 0.f, xm = -__builtin_inff();
+  if (lane < a.K) {
+    mine = a.idx[tok * a.K + lane];
+    dw = a.dweight[tok * a.K + lane];
+  }
+  float x[V], s[V], mx = -__builtin_inff(), sum = 0.f;
+  live_logits<V, VEC>(l, e0, a.E, a.active, x);
+  xm = live_logit(l, mine, a.E, a.active);
+#pragma unroll
+  for (int v = 0; v < V; v++) mx = fmaxf(mx, x[v]);
+  mx = row_max(mx);
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const bool live = x[v] > -__builtin_inff();
+    s[v] = !live ? 0.f : a.score ? 1.f / (1.f + expf(-x[v])) : x[v] == mx ? 1.f : expf(x[v] - mx);
+    sum += s[v];
+  }
+  const float by = a.score ? 1.f : row16_sum(sum);
+  const bool some = xm > -__builtin_inff();  // (false without a choice: mine -1 is not live)
+  mine = some ? mine : -1;
+  float sk = a.score ? 1.f / (1.f + expf(-xm)) : (xm == mx ? 1.f : expf(xm - mx)) / by;
+  sk = some ? sk : 0.f;
+  float u = some ? dw * a.scale : 0.f;
+  if (a.renorm) {
+    const float total = row16_sum(sk), dot = row16_sum(u * sk);
+    u = (int)some & (int)(total > 0.f) ? (u - dot / total) / total : 0.f;
+  }
+  const float dot = a.score ? 0.f : row16_sum(u * sk);
+  float ds[V];
+#pragma unroll
+  for (int v = 0; v < V; v++) ds[v] = 0.f;
+  for (int k = 0; k < a.K; k++) {
+    const int from = (threadIdx.x & 48) + k;
+    const int e = __shfl(mine, from, kWave) - e0;
+    const float d = __shfl(u, from, kWave);
+#pragma unroll
+    for (int v = 0; v < V; v++) ds[v] += e == v ? d : 0.f;
+  }
+  const float p1 = by > 0.f ? 1.f / by : 0.f;  // (0: no expert is live)
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const float p = s[v] * p1;
+    ds[v] = a.score ? p * (1.f - p) * ds[v] : p * (ds[v] - dot);
+  }
+  if (!in) return;
+  float* __restrict__ to = a.dlogits + tok * a.E;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int v = 0; v < V; v += 4)
+      if (e0 + v < a.E) *reinterpret_cast<float4*>(to + e0 + v) = make_float4(ds[v], ds[v + 1], ds[v + 2], ds[v + 3]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; v++)
+      if (e0 + v < a.E) to[e0 + v] = ds[v];
+  }
+}
+
 // ---- slots sorted by expert -------------------------------------------------------
 
 constexpr int kSortBlock = 1024;  // slots a workgroup
@@ -598,12 +857,32 @@ GemmArgs grouped(const Tables& t, int64_t rows, int64_t N, int64_t K, const floa
 
 }  // namespace
 
+static bool rows_of_16(int64_t E, int64_t K) { return E <= 256 && K <= 16; }
+static bool logits_float4(int64_t E, const void* p, const void* q) {
+  return E % 4 == 0 && ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 15) == 0;
+}
+
+#define NSH_ROUTE_ROWS(KERNEL_)                                                                     \
+  do {                                                                                              \
+    const dim3 g((unsigned)ceil_div(a.T, 16));                                                      \
+    if (a.E <= 16) hipLaunchKernelGGL((KERNEL_<1, false>), g, dim3(256), 0, s, a);                  \
+    else if (vec && a.E <= 64) hipLaunchKernelGGL((KERNEL_<4, true>), g, dim3(256), 0, s, a);       \
+    else if (vec && a.E <= 128) hipLaunchKernelGGL((KERNEL_<8, true>), g, dim3(256), 0, s, a);      \
+    else if (vec) hipLaunchKernelGGL((KERNEL_<16, true>), g, dim3(256), 0, s, a);                   \
+    else if (a.E <= 64) hipLaunchKernelGGL((KERNEL_<4, false>), g, dim3(256), 0, s, a);             \
+    else hipLaunchKernelGGL((KERNEL_<16, false>), g, dim3(256), 0, s, a);                           \
+  } while (0)
+
 int launch_route(const RouteArgs& a, hipStream_t s) {
   if (a.T <= 0) return 0;
+  if (rows_of_16(a.E, a.K)) {
+    const bool vec = logits_float4(a.E, a.logits, nullptr);
+    NSH_ROUTE_ROWS(route_row_kernel);
+    NSH_LAUNCHED();
+    return 0;
+  }
   const dim3 g((unsigned)ceil_div(a.T, 4));
-  if (a.E <= 64) hipLaunchKernelGGL(route_kernel<1>, g, dim3(256), 0, s, a);
-  else if (a.E <= 128) hipLaunchKernelGGL(route_kernel<2>, g, dim3(256), 0, s, a);
-  else if (a.E <= 256) hipLaunchKernelGGL(route_kernel<4>, g, dim3(256), 0, s, a);
+  if (a.E <= 256) hipLaunchKernelGGL(route_kernel<4>, g, dim3(256), 0, s, a);
   else if (a.E <= 512) hipLaunchKernelGGL(route_kernel<8>, g, dim3(256), 0, s, a);
   else hipLaunchKernelGGL(route_kernel<16>, g, dim3(256), 0, s, a);
   NSH_LAUNCHED();
@@ -612,10 +891,14 @@ int launch_route(const RouteArgs& a, hipStream_t s) {
 
 int launch_route_grad(const RouteGradArgs& a, hipStream_t s) {
   if (a.T <= 0) return 0;
+  if (rows_of_16(a.E, a.K)) {
+    const bool vec = logits_float4(a.E, a.logits, a.dlogits);
+    NSH_ROUTE_ROWS(route_grad_row_kernel);
+    NSH_LAUNCHED();
+    return 0;
+  }
   const dim3 g((unsigned)ceil_div(a.T, 4));
-  if (a.E <= 64) hipLaunchKernelGGL(route_grad_kernel<1>, g, dim3(256), 0, s, a);
-  else if (a.E <= 128) hipLaunchKernelGGL(route_grad_kernel<2>, g, dim3(256), 0, s, a);
-  else if (a.E <= 256) hipLaunchKernelGGL(route_grad_kernel<4>, g, dim3(256), 0, s, a);
+  if (a.E <= 256) hipLaunchKernelGGL(route_grad_kernel<4>, g, dim3(256), 0, s, a);
   else if (a.E <= 512) hipLaunchKernelGGL(route_grad_kernel<8>, g, dim3(256), 0, s, a);
   else hipLaunchKernelGGL(route_grad_kernel<16>, g, dim3(256), 0, s, a);
   NSH_LAUNCHED();
