@@ -297,6 +297,23 @@ int launch_route_grad(const RouteGradArgs& a, hipStream_t s);
 struct MoeShape {
   int64_t T, K, D, H, E;
 };
+// Slots (token, choice) sorted by expert, stable.
+struct SlotTables {
+  int* seg;            // [E + 1] segments of the sorted order
+  int* perm;           // position -> slot (-1: a padding position)
+  int* tok;            // position -> token (-1)
+  int* expert;         // slot -> expert, -1 where idx is out of range
+  int* tiles;          // (expert, tile of bm rows) pairs
+  int* ntiles;         // how many
+  int* blk = nullptr;  // optional: the expert of every `pad` positions
+};
+int64_t sort_count_ints(int64_t N, int64_t E);
+// Segments start at multiples of `pad`; fill: positions to preset to -1.
+int launch_sort_slots(const int32_t* idx, const SlotTables& t, int* count, int64_t N, int K, int E, int pad, int bm,
+                      int64_t fill, hipStream_t s);
+// y[t] = the sum of the rows o[slot] of the token's slots that have an expert
+int launch_combine(const float* o, const int* expert, float* y, const MoeShape& m, hipStream_t s);
+
 size_t experts_state_bytes(const MoeShape& m);
 size_t experts_workspace_bytes(const MoeShape& m, bool grad);
 int launch_experts(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2, float* y,

@@ -482,10 +482,16 @@ __device__ __forceinline__ int slot_expert(const int32_t* __restrict__ idx, int6
   return e >= 0 && e < E ? e : -1;
 }
 
-// count[block][e]: the block's slots of each expert.
+// count[block][e]: the block's slots of each expert.  fill (not 0): perm and
+// tok of positions 0 .. fill - 1 are set to -1.
 __global__ __launch_bounds__(kSortBlock) void slots_count_kernel(const int32_t* __restrict__ idx, int64_t N, int E,
-                                                                 int* __restrict__ count) {
+                                                                 int* __restrict__ count, int* __restrict__ perm,
+                                                                 int* __restrict__ tok, int64_t fill) {
   __shared__ int c[kMoeMaxExperts];
+  for (int64_t i = (int64_t)blockIdx.x * kSortBlock + threadIdx.x; i < fill; i += (int64_t)gridDim.x * kSortBlock) {
+    perm[i] = -1;
+    tok[i] = -1;
+  }
   for (int e = threadIdx.x; e < E; e += kSortBlock) c[e] = 0;
   __syncthreads();
   const int e = slot_expert(idx, (int64_t)blockIdx.x * kSortBlock + threadIdx.x, N, E);
@@ -495,42 +501,72 @@ __global__ __launch_bounds__(kSortBlock) void slots_count_kernel(const int32_t* 
   for (int i = threadIdx.x; i < E; i += kSortBlock) count[(int64_t)blockIdx.x * E + i] = c[i];
 }
 
-// Each expert's segment, the blocks' offsets in it (in place of their counts)
-// and the (expert, tile of 128 rows) list.  One workgroup, thread e an expert.
-__global__ __launch_bounds__(kMoeMaxExperts) void slots_scan_kernel(int* __restrict__ count, int nblk, int E,
-                                                                    int* __restrict__ seg, int* __restrict__ tiles,
-                                                                    int* __restrict__ ntiles) {
-  __shared__ int n[kMoeMaxExperts], t[kMoeMaxExperts];
-  const int e = threadIdx.x;
+// Inclusive sum over the 1024 threads; `room`: 16 ints.
+__device__ __forceinline__ int block_scan(int v, int* room) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int b = __shfl_up(v, o, kWave);
+    v += lane >= o ? b : 0;
+  }
+  __syncthreads();  // (room's last use)
+  if (lane == 63) room[w] = v;
+  __syncthreads();
+  int before = 0;
+  for (int u = 0; u < w; u++) before += room[u];
+  return before + v;
+}
+
+// Each expert's segment (its start rounded up to `pad` positions), the blocks'
+// offsets in it (in place of their counts), the (expert, tile of bm rows) list
+// and, blk not null, the expert of every `pad` positions.  One workgroup: thread
+// (part, expert) sums a run of blocks, then the sums of all (expert, part) are
+// scanned in that order.
+__global__ __launch_bounds__(1024) void slots_scan_kernel(int* __restrict__ count, int nblk, int E, int pad, int bm,
+                                                          int* __restrict__ seg, int* __restrict__ tiles,
+                                                          int* __restrict__ ntiles, int* __restrict__ blk) {
+  __shared__ int sum[1024], before[1024], start[1024], room[16];
+  const int t = threadIdx.x;
+  int ep = 1;
+  while (ep < E) ep <<= 1;
+  const int parts = 1024 / ep, e = t & (ep - 1), part = t / ep;
+  const int run = (nblk + parts - 1) / parts, b0 = min(nblk, part * run), b1 = min(nblk, b0 + run);
+  int c = 0;
+  if (e < E) {
+#pragma unroll 8
+    for (int b = b0; b < b1; b++) c += count[(int64_t)b * E + e];
+  }
+  sum[e * parts + part] = c;
+  __syncthreads();
+  const int v = sum[t];
+  before[t] = block_scan(v, room) - v;
+  __syncthreads();
+  // thread e: its expert's total, segment and tiles
   int total = 0;
-  if (e < E)
-    for (int b = 0; b < nblk; b++) total += count[(int64_t)b * E + e];
-  n[e] = total;
-  t[e] = (total + 127) / 128;
-  for (int o = 1; o < kMoeMaxExperts; o <<= 1) {
-    __syncthreads();
-    const int pn = e >= o ? n[e - o] : 0, pt = e >= o ? t[e - o] : 0;
-    __syncthreads();
-    n[e] += pn;
-    t[e] += pt;
+  if (t < E) total = (t + 1 < ep ? before[(t + 1) * parts] : before[1023] + sum[1023]) - before[t * parts];
+  const int padded = (total + pad - 1) / pad * pad, nt = (total + bm - 1) / bm;
+  const int at = block_scan(padded, room) - padded, ta = block_scan(nt, room) - nt;
+  if (t < E) {
+    start[t] = at;
+    seg[t] = at;
+    if (t == E - 1) {
+      seg[E] = at + padded;
+      *ntiles = ta + nt;
+    }
+    for (int i = 0; i < nt; i++) {
+      tiles[2 * (ta + i)] = t;
+      tiles[2 * (ta + i) + 1] = i;
+    }
+    if (blk)
+      for (int i = 0; i < padded / pad; i++) blk[at / pad + i] = t;
   }
   __syncthreads();
   if (e >= E) return;
-  const int nt = (total + 127) / 128;
-  int at = n[e] - total;
-  seg[e] = at;
-  if (e == E - 1) {
-    seg[E] = n[e];
-    *ntiles = t[e];
-  }
-  for (int b = 0; b < nblk; b++) {
-    const int c = count[(int64_t)b * E + e];
-    count[(int64_t)b * E + e] = at;
-    at += c;
-  }
-  for (int i = 0; i < nt; i++) {
-    tiles[2 * (t[e] - nt + i)] = e;
-    tiles[2 * (t[e] - nt + i) + 1] = i;
+  int off = start[e] + before[e * parts + part] - before[e * parts];
+  for (int b = b0; b < b1; b++) {
+    const int n = count[(int64_t)b * E + e];
+    count[(int64_t)b * E + e] = off;
+    off += n;
   }
 }
 
@@ -800,15 +836,12 @@ __global__ __launch_bounds__(256) void few_combine_kernel(const float* __restric
   y[i] = y0;
 }
 
-struct Tables {
-  int *seg, *perm, *tok, *expert, *tiles, *ntiles;
-};
 constexpr int64_t round64(int64_t n) { return (n + 63) / 64 * 64; }
 int64_t tables_ints(int64_t N, int64_t E) {
   return round64(E + 1) + 3 * round64(N) + round64(2 * (ceil_div(N, 128) + E)) + 64;
 }
-Tables tables_at(int* p, int64_t N, int64_t E) {
-  Tables t;
+SlotTables tables_at(int* p, int64_t N, int64_t E) {
+  SlotTables t;
   t.seg = p;
   t.perm = t.seg + round64(E + 1);
   t.tok = t.perm + round64(N);
@@ -817,34 +850,10 @@ Tables tables_at(int* p, int64_t N, int64_t E) {
   t.ntiles = t.tiles + round64(2 * (ceil_div(N, 128) + E));
   return t;
 }
-int64_t count_ints(int64_t N, int64_t E) { return round64(ceil_div(N, kSortBlock) * E); }
-
-int sort_slots(const int32_t* idx, const Tables& t, int* count, int64_t N, int K, int E, hipStream_t s) {
-  const int nblk = (int)ceil_div(N, kSortBlock);
-  hipLaunchKernelGGL(slots_count_kernel, dim3(nblk), dim3(kSortBlock), 0, s, idx, N, E, count);
-  NSH_LAUNCHED();
-  hipLaunchKernelGGL(slots_scan_kernel, dim3(1), dim3(kMoeMaxExperts), 0, s, count, nblk, E, t.seg, t.tiles, t.ntiles);
-  NSH_LAUNCHED();
-  hipLaunchKernelGGL(slots_place_kernel, dim3(nblk), dim3(kSortBlock), 0, s, idx, N, E, K, count, t.perm, t.tok,
-                     t.expert);
-  NSH_LAUNCHED();
-  return 0;
-}
 
 unsigned stream_blocks(int64_t n) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(n, 256), 8192)); }
 
-int launch_combine(const float* o, const int* expert, float* y, const MoeShape& m, hipStream_t s) {
-  if (m.D % 4 == 0 && ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(y)) & 15) == 0)
-    hipLaunchKernelGGL(combine_kernel<4>, dim3(stream_blocks(m.T * m.D / 4)), dim3(256), 0, s, o, expert, y, m.T,
-                       (int)m.K, m.D / 4);
-  else
-    hipLaunchKernelGGL(combine_kernel<1>, dim3(stream_blocks(m.T * m.D)), dim3(256), 0, s, o, expert, y, m.T, (int)m.K,
-                       m.D);
-  NSH_LAUNCHED();
-  return 0;
-}
-
-GemmArgs grouped(const Tables& t, int64_t rows, int64_t N, int64_t K, const float* A, const float* B, float* C,
+GemmArgs grouped(const SlotTables& t, int64_t rows, int64_t N, int64_t K, const float* A, const float* B, float* C,
                  const MoeShape& m, bool tB) {
   GemmArgs g;
   g.A = A; g.B = B; g.C = C;
@@ -872,6 +881,33 @@ static bool logits_float4(int64_t E, const void* p, const void* q) {
     else if (a.E <= 64) hipLaunchKernelGGL((KERNEL_<4, false>), g, dim3(256), 0, s, a);             \
     else hipLaunchKernelGGL((KERNEL_<16, false>), g, dim3(256), 0, s, a);                           \
   } while (0)
+
+int launch_combine(const float* o, const int* expert, float* y, const MoeShape& m, hipStream_t s) {
+  if (m.D % 4 == 0 && ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(y)) & 15) == 0)
+    hipLaunchKernelGGL(combine_kernel<4>, dim3(stream_blocks(m.T * m.D / 4)), dim3(256), 0, s, o, expert, y, m.T,
+                       (int)m.K, m.D / 4);
+  else
+    hipLaunchKernelGGL(combine_kernel<1>, dim3(stream_blocks(m.T * m.D)), dim3(256), 0, s, o, expert, y, m.T, (int)m.K,
+                       m.D);
+  NSH_LAUNCHED();
+  return 0;
+}
+
+int64_t sort_count_ints(int64_t N, int64_t E) { return round64(ceil_div(N, kSortBlock) * E); }
+
+int launch_sort_slots(const int32_t* idx, const SlotTables& t, int* count, int64_t N, int K, int E, int pad, int bm,
+                      int64_t fill, hipStream_t s) {
+  const int nblk = (int)ceil_div(N, kSortBlock);
+  hipLaunchKernelGGL(slots_count_kernel, dim3(nblk), dim3(kSortBlock), 0, s, idx, N, E, count, t.perm, t.tok, fill);
+  NSH_LAUNCHED();
+  hipLaunchKernelGGL(slots_scan_kernel, dim3(1), dim3(1024), 0, s, count, nblk, E, pad, bm, t.seg, t.tiles, t.ntiles,
+                     t.blk);
+  NSH_LAUNCHED();
+  hipLaunchKernelGGL(slots_place_kernel, dim3(nblk), dim3(kSortBlock), 0, s, idx, N, E, K, count, t.perm, t.tok,
+                     t.expert);
+  NSH_LAUNCHED();
+  return 0;
+}
 
 int launch_route(const RouteArgs& a, hipStream_t s) {
   if (a.T <= 0) return 0;
@@ -961,7 +997,7 @@ size_t experts_state_bytes(const MoeShape& m) {
 // sorted and the slots [N, D], and the weight gradients' items and partial sums
 size_t experts_workspace_bytes(const MoeShape& m, bool grad) {
   const int64_t N = m.T * m.K;
-  const int64_t fwd = count_ints(N, m.E) + tables_ints(N, m.E) + round64(N * m.H) + N * m.D;
+  const int64_t fwd = sort_count_ints(N, m.E) + tables_ints(N, m.E) + round64(N * m.H) + N * m.D;
   const int64_t bwd = 2 * round64(N * m.H) + 3 * round64(N * m.D) + round64(moe_bwd_kpart_floats(N, m.D, m.H)) +
                       moe_bwd_kitem_ints(N, m.D, m.H, m.E);
   const int64_t few = few_slots(m) ? round64(few_chunks(m.D, m.H, N, m.E) * N * m.H) +
@@ -977,13 +1013,13 @@ int launch_experts(const float* x, const int32_t* idx, const float* weight, cons
   if (!state && few_slots(m)) return launch_few(x, idx, weight, W1, W2, y, m, act, workspace, s);
   int* wi = static_cast<int*>(workspace);
   int* count = wi;
-  wi += count_ints(N, m.E);
+  wi += sort_count_ints(N, m.E);
   int* ti = state ? static_cast<int*>(state) : wi;
   if (!state) wi += tables_ints(N, m.E);
   float* hidden = reinterpret_cast<float*>(wi);
   float* slots = hidden + round64(N * m.H);
-  const Tables t = tables_at(ti, N, m.E);
-  if (sort_slots(idx, t, count, N, (int)m.K, (int)m.E, s) != 0) return -1;
+  const SlotTables t = tables_at(ti, N, m.E);
+  if (launch_sort_slots(idx, t, count, N, (int)m.K, (int)m.E, 1, 128, 0, s) != 0) return -1;
   GemmArgs g = grouped(t, N, m.H, m.D, x, W1, hidden, m, false);
   g.a_rows = t.tok;
   g.act = act;
@@ -1009,7 +1045,7 @@ int launch_experts_grad(const float* dy, const float* x, const float* weight, co
     return dweight ? launch_fill(dweight, N, 0.f, s) : 0;
   }
   int* ti = const_cast<int*>(static_cast<const int*>(state));
-  const Tables t = tables_at(ti, N, m.E);
+  const SlotTables t = tables_at(ti, N, m.E);
   const float* pre = reinterpret_cast<const float*>(ti + tables_ints(N, m.E));
   float* dh = static_cast<float*>(workspace);
   float* hw = dh + round64(N * m.H);
