@@ -247,6 +247,11 @@ int launch_moe_kitems(const int* seg, int* kitems, int* dirty, int64_t M, int64_
                       hipStream_t s);
 int launch_moe_weight_grad(const float* A, const float* B, float* C, int64_t R, int64_t Cc, const int* kitems,
                            float* kpart, int64_t M, int64_t D, int64_t H, int64_t E, hipStream_t s);
+// Most items that launch_moe_kitems makes, and the sum of the items' partial
+// results kpart into the C[e] (DH floats each) of experts with several.
+int64_t moe_bwd_most_items(int64_t M, int64_t D, int64_t H, int64_t E);
+int launch_moe_kpart_sum(float* C, int64_t DH, const int* kitems, const float* kpart, int64_t M, int64_t D, int64_t H,
+                         int64_t E, hipStream_t s);
 size_t moe_work_ints(int64_t M, int64_t E);   // int-sized words of all int arrays
 int launch_moe_route(const float* x, const float* Wg, const uint8_t* active, const MoeWork& w, int64_t M, int64_t D,
                      int64_t E, hipStream_t s);
@@ -321,6 +326,17 @@ int launch_experts(const float* x, const int32_t* idx, const float* weight, cons
 int launch_experts_grad(const float* dy, const float* x, const float* weight, const float* W1, const float* W2,
                         const void* state, float* dx, float* dweight, float* dW1, float* dW2, const MoeShape& m,
                         int act, void* workspace, hipStream_t s);
+
+// moe_split.hip: the same for layers that split_takes (by their sizes alone, so
+// that the gradient follows its forward).
+bool split_takes(const MoeShape& m);
+size_t split_state_bytes(const MoeShape& m);
+size_t split_workspace_bytes(const MoeShape& m, bool grad);
+int launch_experts_split(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2,
+                         float* y, const MoeShape& m, int act, void* state, void* workspace, hipStream_t s);
+int launch_experts_split_grad(const float* dy, const float* x, const float* weight, const float* W1, const float* W2,
+                              const void* state, float* dx, float* dweight, float* dW1, float* dW2, const MoeShape& m,
+                              int act, void* workspace, hipStream_t s);
 
 // newton.hip -------------------------------------------------------------------
 // Orthogonalisation of n matrices [r, c] by `steps` Newton-Schulz products.

@@ -926,29 +926,34 @@ int launch_moe_kitems(const int* seg, int* kitems, int* dirty, int64_t M, int64_
   return 0;
 }
 
+int64_t moe_bwd_most_items(int64_t M, int64_t D, int64_t H, int64_t E) { return kitems_max(M, D, H, E); }
+
+int launch_moe_kpart_sum(float* C, int64_t DH, const int* kitems, const float* kpart, int64_t M, int64_t D, int64_t H,
+                         int64_t E, hipStream_t s) {
+  const int maxitems = (int)kitems_max(M, D, H, E), maxred = (int)kreduce_max(M, D, H);
+  if (maxred <= 0) return 0;
+  const bool vec = DH % 4 == 0 && ((reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(kpart)) & 15) == 0;
+  // one element (float4) per thread: each entry's sum is a few MB, and
+  // fewer threads looping over it left the pass latency-bound
+  const unsigned gx = (unsigned)std::min<int64_t>(ceil_div(vec ? DH / 4 : DH, 256), 4096);
+  if (vec)
+    hipLaunchKernelGGL(moe_kpart_sum_kernel<true>, dim3(gx, maxred), dim3(256), 0, s, kitems, maxitems, kpart, C, DH);
+  else
+    hipLaunchKernelGGL(moe_kpart_sum_kernel<false>, dim3(gx, maxred), dim3(256), 0, s, kitems, maxitems, kpart, C, DH);
+  NSH_LAUNCHED();
+  return 0;
+}
+
 int launch_moe_weight_grad(const float* A, const float* B, float* C, int64_t R, int64_t Cc, const int* kitems,
                            float* kpart, int64_t M, int64_t D, int64_t H, int64_t E, hipStream_t s) {
-  const int maxitems = (int)kitems_max(M, D, H, E), maxred = (int)kreduce_max(M, D, H);
   GemmArgs k;
   k.A = A; k.B = B; k.C = C;
   k.M = (int)R; k.N = (int)Cc; k.K = (int)M;
   k.lda = R; k.ldb = Cc; k.ldc = Cc;
   k.sC = R * Cc;
   k.kitems = kitems + 2; k.nkitems = kitems; k.kpart = kpart;
-  if (launch_gemm_ex(k, true, false, maxitems, s) != 0) return -1;
-  if (maxred > 0) {
-    const int64_t DH = R * Cc;
-    const bool vec = DH % 4 == 0 && ((reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(kpart)) & 15) == 0;
-    // one element (float4) per thread: each entry's sum is a few MB, and
-    // fewer threads looping over it left the pass latency-bound
-    const unsigned gx = (unsigned)std::min<int64_t>(ceil_div(vec ? DH / 4 : DH, 256), 4096);
-    if (vec)
-      hipLaunchKernelGGL(moe_kpart_sum_kernel<true>, dim3(gx, maxred), dim3(256), 0, s, kitems, maxitems, kpart, C, DH);
-    else
-      hipLaunchKernelGGL(moe_kpart_sum_kernel<false>, dim3(gx, maxred), dim3(256), 0, s, kitems, maxitems, kpart, C, DH);
-    NSH_LAUNCHED();
-  }
-  return 0;
+  if (launch_gemm_ex(k, true, false, (int)kitems_max(M, D, H, E), s) != 0) return -1;
+  return launch_moe_kpart_sum(C, R * Cc, kitems, kpart, M, D, H, E, s);
 }
 
 // dWg[D, E] = x[M, D]^T dg[M, E]

@@ -14,6 +14,7 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "moe_act.h"
 
 namespace nship {
 namespace {
@@ -617,14 +618,6 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
   }
 }
 
-// act'(u).  SiLU's is sigma (1 + u (1 - sigma)); the networks' own layers take
-// the reference's spelling (act_deriv), which is another function.
-__device__ __forceinline__ float act_slope(float u, int act) {
-  if (act != kActSilu) return act_deriv(u, act);
-  const float s = 1.f / (1.f + expf(-u));
-  return s + u * s * (1.f - s);
-}
-
 // One wave per sorted row: dweight = act(u) . dh, du = weight act'(u) dh (in
 // place of dh), hw = weight act(u).
 __global__ __launch_bounds__(256) void bwd_rows_kernel(const float* __restrict__ pre, float* __restrict__ dh,
@@ -989,6 +982,7 @@ static int launch_few(const float* x, const int32_t* idx, const float* weight, c
 
 // state: the sorted slots' tables, then the pre-activations [T K, H]
 size_t experts_state_bytes(const MoeShape& m) {
+  if (split_takes(m)) return split_state_bytes(m);
   const int64_t N = m.T * m.K;
   return 4 * (size_t)(tables_ints(N, m.E) + N * m.H);
 }
@@ -996,6 +990,7 @@ size_t experts_state_bytes(const MoeShape& m) {
 // hidden [N, H] and slots [N, D]; of the backward dh, hw [N, H], x and dy
 // sorted and the slots [N, D], and the weight gradients' items and partial sums
 size_t experts_workspace_bytes(const MoeShape& m, bool grad) {
+  if (split_takes(m)) return split_workspace_bytes(m, grad);
   const int64_t N = m.T * m.K;
   const int64_t fwd = sort_count_ints(N, m.E) + tables_ints(N, m.E) + round64(N * m.H) + N * m.D;
   const int64_t bwd = 2 * round64(N * m.H) + 3 * round64(N * m.D) + round64(moe_bwd_kpart_floats(N, m.D, m.H)) +
@@ -1010,6 +1005,7 @@ int launch_experts(const float* x, const int32_t* idx, const float* weight, cons
                    const MoeShape& m, int act, void* state, void* workspace, hipStream_t s) {
   const int64_t N = m.T * m.K;
   if (m.T <= 0 || m.D <= 0) return 0;
+  if (split_takes(m)) return launch_experts_split(x, idx, weight, W1, W2, y, m, act, state, workspace, s);
   if (!state && few_slots(m)) return launch_few(x, idx, weight, W1, W2, y, m, act, workspace, s);
   int* wi = static_cast<int*>(workspace);
   int* count = wi;
@@ -1044,6 +1040,8 @@ int launch_experts_grad(const float* dy, const float* x, const float* weight, co
     if (dW2 && launch_fill(dW2, m.E * m.D * m.H, 0.f, s) != 0) return -1;
     return dweight ? launch_fill(dweight, N, 0.f, s) : 0;
   }
+  if (split_takes(m))
+    return launch_experts_split_grad(dy, x, weight, W1, W2, state, dx, dweight, dW1, dW2, m, act, workspace, s);
   int* ti = const_cast<int*>(static_cast<const int*>(state));
   const SlotTables t = tables_at(ti, N, m.E);
   const float* pre = reinterpret_cast<const float*>(ti + tables_ints(N, m.E));

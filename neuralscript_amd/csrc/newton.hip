@@ -11,51 +11,32 @@
 // and 2 m^2 N FLOP; bound by the matrix cores from some hundred rows on, below
 // by launches and the latency of a slab's loads.
 //
-// Products of two fp16 pieces.  The map keeps |X| and |S| (entries and singular
-// values) below 1.21^2 and |P| below 3.45 whatever G is, so one power of two
-// per operand puts every entry into fp16's range, and v = h + l with h =
-// fp16(v), l = fp16(v - h) holds 22 bits of it (23 with l's sign): two fp16
-// MFMA operands instead of split3.h's three bf16 ones, and three products h h,
-// h l, l h instead of six.  What that drops: 2^-23 of an operand at most (fp32:
-// 2^-24), l l below 2^-22 of a product, and of entries below 2^-18 the bits
-// under 2^-40.  Rounding at random, that is 2^-23.6 of a product, against the
-// 10 x 2^-24 and more that fp32 sums of 1024 terms lose; measured errors are
-// in the table of launch_newton_schulz.
+// Products of two fp16 pieces (split2.h).  The map keeps |X| and |S| (entries and
+// singular values) below 1.21^2 and |P| below 3.45 whatever G is, so one power of
+// two per operand puts every entry into fp16's range.  Measured against 64 bits,
+// relative, fp32 products and these: 8 of 64 x 256 1.4e-6, 1.4e-6; 1000 x 333
+// 2.7e-6, 1.3e-6.
 //
 // The norm's 1e-7 leaves X0 small where G is.  X is then held times 2^e, e = e0 -
 // 2 k at step k and not below 0 (a step grows X by at most 3.4445), so that its
 // entries keep their bits.
 //
-// Layout.  An operand with rows R and contraction length K is stored as
-// [piece][K / 8][R][8]: the 16-byte chunk of 8 consecutive k of one row is what
-// one lane of an MFMA takes, and a slab of a tile is contiguous runs of chunks,
-// copied to LDS as they lie.  K is padded with zeros to a multiple of 32.  X is
-// kept both ways, as the Gram product's operand (rows m, contraction N) and as
+// Operands are padded with zeros to a contraction length of 32 k.  X is kept both ways, as the Gram product's operand (rows m, contraction N) and as
 // the update's (rows N, contraction m); S and P are symmetric and need one.
 #include <algorithm>
 
 #include "common.h"
 #include "kernels.h"
+#include "split2.h"
 
 namespace nship {
 namespace {
-
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
 constexpr double kNsEps = 1e-7;
 constexpr int kNormParts = 64;  // partial sums of a matrix's norm
 // the operands' powers of two: X and S below 2 x 2^15 = fp16's range, P below 4 x 2^14
 constexpr float kUpX = 0x1p15f, kUpS = 0x1p15f, kUpP = 0x1p14f;
-
-__device__ __forceinline__ void split2(float v, _Float16& h, _Float16& l) {
-  h = (_Float16)v;
-  l = (_Float16)(v - (float)h);
-}
 
 // What a product is for, i.e. its epilogue.
 enum NsMode : int { kGram = 0, kPoly, kUpdate, kLast };
@@ -78,11 +59,6 @@ struct NsArgs {
   const int* ex;       // e0 of every matrix
   int step;
 };
-
-__device__ __forceinline__ int ns_xcd_linear(int b, int T) {
-  const int per = T >> 3, rem = T & 7, x = b & 7, i = b >> 3;
-  return x * per + (x < rem ? x : rem) + i;
-}
 
 // Tile of linear index t: by rows, or of a lower triangle (tn <= tm) by rows.
 template <bool SYM>
@@ -199,117 +175,27 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& g, const floatx16 (&ac
   }
 }
 
-// One tile of C = A B^T: WM x WN waves of TM x TN blocks of 32x32, slabs of KS.
+// One tile of C = A B^T (split2.h).
 template <int MODE, int WM, int WN, int TM, int TN, int KS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void ns_gemm_kernel(NsArgs g) {
-  constexpr int NT = 64 * WM * WN, RA = 32 * WM * TM, RB = 32 * WN * TN, OCT = KS / 8;
-  constexpr int CA = 2 * OCT * RA / NT, CB = 2 * OCT * RB / NT;  // chunks a thread
-  constexpr int kBuf = 2 * OCT * (RA + RB) * 16;
-  static_assert(CA * NT == 2 * OCT * RA && CB * NT == 2 * OCT * RB, "the chunks divide evenly");
-  static_assert(kTurnBytes * WM * WN <= 2 * kBuf, "the transposing tiles fit");
+  using Tile = Split2Tile<WM, WN, TM, TN, KS>;
+  static_assert(kTurnBytes * WM * WN <= Tile::kLds, "the transposing tiles fit");
   constexpr bool kSym = MODE == kGram || MODE == kPoly;
-  __shared__ __attribute__((aligned(16))) char smem[2 * kBuf];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int wm = wave / WN, wn = wave % WN, l32 = lane & 31, kh = lane >> 5;
-  const int L = ns_xcd_linear(blockIdx.x, g.tiles * g.n);
+  static_assert(!kSym || Tile::RA == Tile::RB, "a symmetric result's tiles are square");
+  __shared__ __attribute__((aligned(16))) char smem[Tile::kLds];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / WN, wn = wave % WN;
+  const int L = split2_xcd_linear(blockIdx.x, g.tiles * g.n);
   const int mat = L / g.tiles;
   int tm, tn;
   ns_tile<kSym>(L % g.tiles, g.tiles_n, tm, tn);
-  const int64_t m0 = (int64_t)tm * RA, n0 = (int64_t)tn * RB;
+  const int64_t m0 = (int64_t)tm * Tile::RA, n0 = (int64_t)tn * Tile::RB;
   floatx16 acc[TM][TN];
-#pragma unroll
-  for (int r = 0; r < TM; r++)
-#pragma unroll
-    for (int c = 0; c < TN; c++)
-#pragma unroll
-      for (int v = 0; v < 16; v++) acc[r][c][v] = 0.f;
-  {
-    // chunk i of thread t: (piece, octet, row), row fastest; rows past the end
-    // read the last one's (their results are not stored)
-    const uintx4* pa[CA];
-    const uintx4* pb[CB];
-#pragma unroll
-    for (int i = 0; i < CA; i++) {
-      const int c = t + NT * i, row = c % RA, o = c / RA % OCT, p = c / RA / OCT;
-      pa[i] = reinterpret_cast<const uintx4*>(g.A + mat * g.sA) + (p * (g.k / 8) + o) * g.ra +
-              min(m0 + row, g.ra - 1);
-    }
-#pragma unroll
-    for (int i = 0; i < CB; i++) {
-      const int c = t + NT * i, row = c % RB, o = c / RB % OCT, p = c / RB / OCT;
-      pb[i] = reinterpret_cast<const uintx4*>(g.B + mat * g.sB) + (p * (g.k / 8) + o) * g.rb +
-              min(n0 + row, g.rb - 1);
-    }
-    const int64_t stepa = OCT * g.ra, stepb = OCT * g.rb;
-    const int nk = (int)(g.k / KS);
-    uintx4 va[2][CA], vb[2][CB];
-    int next = 0;  // slab to load; past the last it is loaded again
-    auto load = [&](auto z) {
-      constexpr int Z = decltype(z)::value;
-#pragma unroll
-      for (int i = 0; i < CA; i++) va[Z][i] = *pa[i];
-#pragma unroll
-      for (int i = 0; i < CB; i++) vb[Z][i] = *pb[i];
-      const bool more = ++next < nk;
-#pragma unroll
-      for (int i = 0; i < CA; i++) pa[i] += more ? stepa : 0;
-#pragma unroll
-      for (int i = 0; i < CB; i++) pb[i] += more ? stepb : 0;
-    };
-    auto store = [&](auto z, char* to) {
-      constexpr int Z = decltype(z)::value;
-#pragma unroll
-      for (int i = 0; i < CA; i++) *reinterpret_cast<uintx4*>(to + (t + NT * i) * 16) = va[Z][i];
-#pragma unroll
-      for (int i = 0; i < CB; i++) *reinterpret_cast<uintx4*>(to + 2 * OCT * RA * 16 + (t + NT * i) * 16) = vb[Z][i];
-    };
-    using Even = std::integral_constant<int, 0>;
-    using Odd = std::integral_constant<int, 1>;
-    load(Even{});
-    load(Odd{});
-    store(Even{}, smem);
-    load(Even{});
-    __syncthreads();
-    auto slab = [&](int kt, auto z) {
-      const char* as = smem + (kt & 1) * kBuf + (kh * RA + wm * TM * 32 + l32) * 16;
-      const char* bs = smem + (kt & 1) * kBuf + 2 * OCT * RA * 16 + (kh * RB + wn * TN * 32 + l32) * 16;
-#pragma unroll
-      for (int s = 0; s < KS / 16; s++) {
-        half8 fa[TM][2], fb[TN][2];
-#pragma unroll
-        for (int c = 0; c < TN; c++)
-#pragma unroll
-          for (int p = 0; p < 2; p++)
-            fb[c][p] = *reinterpret_cast<const half8*>(bs + ((p * OCT + 2 * s) * RB + c * 32) * 16);
-#pragma unroll
-        for (int r = 0; r < TM; r++)
-#pragma unroll
-          for (int p = 0; p < 2; p++)
-            fa[r][p] = *reinterpret_cast<const half8*>(as + ((p * OCT + 2 * s) * RA + r * 32) * 16);
-#pragma unroll
-        for (int r = 0; r < TM; r++) {
-#pragma unroll
-          for (int c = 0; c < TN; c++)
-            acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[r][1], fb[c][0], acc[r][c], 0, 0, 0);
-#pragma unroll
-          for (int c = 0; c < TN; c++)
-            acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[r][0], fb[c][1], acc[r][c], 0, 0, 0);
-#pragma unroll
-          for (int c = 0; c < TN; c++)
-            acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[r][0], fb[c][0], acc[r][c], 0, 0, 0);
-        }
-      }
-      store(z, smem + ((kt + 1) & 1) * kBuf);
-      load(z);
-      __syncthreads();
-    };
-    for (int kt = 0; kt < nk; kt += 2) {
-      slab(kt, Odd{});
-      if (kt + 1 < nk) slab(kt + 1, Even{});
-    }
-  }
-  ns_epilogue<MODE, TM, TN>(g, acc, smem + wave * kTurnBytes, mat, m0 + wm * TM * 32, n0 + wn * TN * 32, l32, kh,
-                            kSym && tm == tn);
+  const Split2Operand A{reinterpret_cast<const uintx4*>(g.A + mat * g.sA), g.ra, g.k / 8 * g.ra, m0, g.ra - 1};
+  const Split2Operand B{reinterpret_cast<const uintx4*>(g.B + mat * g.sB), g.rb, g.k / 8 * g.rb, n0, g.rb - 1};
+  Tile::run(A, B, (int)(g.k / KS), smem, acc);
+  ns_epilogue<MODE, TM, TN>(g, acc, smem + wave * kTurnBytes, mat, m0 + wm * TM * 32, n0 + wn * TN * 32, lane & 31,
+                            lane >> 5, kSym && tm == tn);
 }
 
 // The same product where larger tiles leave most CUs idle: 32 x 32 outputs a
@@ -326,7 +212,7 @@ __global__ __launch_bounds__(512) void ns_few_kernel(NsArgs g) {
   __shared__ __attribute__((aligned(16))) float part[7][1024];
   const int t = threadIdx.x, lane = t & 63, l32 = lane & 31, kh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int L = ns_xcd_linear(blockIdx.x, g.tiles * g.n);
+  const int L = split2_xcd_linear(blockIdx.x, g.tiles * g.n);
   const int mat = L / g.tiles;
   int tm, tn;
   ns_tile<kSym>(L % g.tiles, g.tiles_n, tm, tn);
