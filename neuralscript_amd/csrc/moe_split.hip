@@ -36,8 +36,10 @@
 namespace nship {
 namespace {
 
-using Tile = Split2Tile<2, 4, 4, 2, 16>;  // 256 x 256
-constexpr int kTM = 4, kTN = 2, kWaves = 8;
+// 256 rows x 128 columns, two workgroups on a CU: one's epilogue runs beside the
+// other's products (256 x 256 and one workgroup of eight waves: TODO).
+constexpr int kTM = 4, kTN = 2, kWM = 2, kWN = 2, kWaves = kWM * kWN;
+using Tile = Split2Tile<kWM, kWN, kTM, kTN, 16>;
 constexpr int kPad = 32;      // positions a segment is padded to
 constexpr int kNoExp = -300;  // "the logarithm of 0"
 constexpr int kPitch = 40;    // halves of a transposing tile's row
@@ -99,117 +101,177 @@ struct RowsArgs {
   int64_t rows, K, Kp;
   int per_expert;     // rows an expert (weights): norm[r / per_expert] is the largest norm instead
 };
-template <bool VEC>
+// Lane (row, part) of a wave's 8 rows takes the octets part, part + 8, .. of its
+// row: 256-byte runs of eight rows are read, 128-byte runs of chunks written.
+// REGS: a row's share stays in registers (K up to 1024), else it is read twice.
+constexpr int kRowOctets = 16;  // octets a lane
+template <bool VEC, bool REGS>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
-  __shared__ int se[32];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, part = lane >> 3;
   const int64_t r0 = (int64_t)blockIdx.x * 32;
   if (a.nrows && r0 >= *a.nrows) return;
-  int big_e = kNoExp, big_n = kNoExp;  // this wave's largest -exponent and norm + weight
-  for (int i = 0; i < 8; i++) {
-    const int64_t r = r0 + w * 8 + i;
-    const int64_t from = r >= a.rows ? -1 : a.tok ? (int64_t)a.tok[r] : r;
-    float top = 0.f;
-    double sq = 0.;
-    if (from >= 0) {  // (uniform per wave)
-      const float* __restrict__ p = a.src + from * a.K;
-      if (VEC) {
-        for (int64_t k = lane * 4; k < a.K; k += 256) {
-          const float4 f = *reinterpret_cast<const float4*>(p + k);
-          const float v[4] = {finite_abs(f.x), finite_abs(f.y), finite_abs(f.z), finite_abs(f.w)};
-#pragma unroll
-          for (int u = 0; u < 4; u++) {
-            top = fmaxf(top, v[u]);
-            sq += (double)v[u] * v[u];
-          }
-        }
-      } else {
-        for (int64_t k = lane; k < a.K; k += 64) {
-          const float v = finite_abs(p[k]);
-          top = fmaxf(top, v);
-          sq += (double)v * v;
-        }
-      }
-    }
-    top = wave_max(top);
-    sq = wave_sum(sq);
-    const int e = row_exp(top), n = log2_norm(sq);
-    if (lane == 0) {
-      se[w * 8 + i] = e;
-      if (r < a.rows) {
-        a.exps[r] = e;
-        if (a.per_expert) atomicMax(&a.norm[r / a.per_expert], n);
-        else a.norm[r] = n;
-        if (from >= 0 && top > 0.f) big_e = max(big_e, -e);
-        if (from >= 0 && a.weight) {
-          const float wt = finite_abs(a.weight[a.perm[r]]);
-          if (wt > 0.f && n > kNoExp) big_n = max(big_n, n + log2_up(wt));
-        }
-      }
-    }
-  }
-  if (a.blk && lane == 0) {
-    const int e = a.blk[blockIdx.x];
-    if (a.top && big_e > kNoExp) atomicMax(&a.top[e], big_e);
-    if (a.wnorm && big_n > kNoExp) atomicMax(&a.wnorm[e], big_n);
-  }
-  __syncthreads();
-  const int row = t & 31;
-  const int64_t r = r0 + row;
-  if (r >= a.rows) return;
-  const int64_t from = a.tok ? (int64_t)a.tok[r] : r;
+  const int64_t r = r0 + w * 8 + (lane & 7);
+  const bool in = r < a.rows;
+  const int64_t from = !in ? -1 : a.tok ? (int64_t)a.tok[r] : r;
   const float* __restrict__ p = a.src + (from >= 0 ? from : 0) * a.K;
-  const int ex = se[row];
-  const int64_t piece = a.Kp * a.rows;
-  for (int64_t o = t >> 5; o < a.Kp / 8; o += 8) {
-    float v[8];
+  const int oct = (int)(a.Kp / 8);
+  auto load = [&](int o, float (&v)[8]) {
     if (VEC) {
 #pragma unroll
       for (int u = 0; u < 8; u += 4) {
-        const bool in = from >= 0 && o * 8 + u < a.K;
-        const float4 f = *reinterpret_cast<const float4*>(p + (in ? o * 8 + u : 0));
-        v[u] = in ? f.x : 0.f; v[u + 1] = in ? f.y : 0.f; v[u + 2] = in ? f.z : 0.f; v[u + 3] = in ? f.w : 0.f;
+        const bool ok = from >= 0 && o * 8 + u < a.K;
+        const float4 f = *reinterpret_cast<const float4*>(p + (ok ? o * 8 + u : 0));
+        v[u] = ok ? f.x : 0.f; v[u + 1] = ok ? f.y : 0.f; v[u + 2] = ok ? f.z : 0.f; v[u + 3] = ok ? f.w : 0.f;
       }
     } else {
 #pragma unroll
       for (int u = 0; u < 8; u++) {
-        const bool in = from >= 0 && o * 8 + u < a.K;
-        const float f = p[in ? o * 8 + u : 0];
-        v[u] = in ? f : 0.f;
+        const bool ok = from >= 0 && o * 8 + u < a.K;
+        const float f = p[ok ? o * 8 + u : 0];
+        v[u] = ok ? f : 0.f;
       }
     }
+  };
+  float top = 0.f;
+  double sq = 0.;
+  auto look = [&](const float (&v)[8]) {
+    float s[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      s[u] = finite_abs(v[u]);
+      top = fmaxf(top, s[u]);
+      sq += (double)s[u] * s[u];
+    }
+  };
+  float keep[REGS ? kRowOctets : 1][8];
+  if constexpr (REGS) {
+#pragma unroll
+    for (int i = 0; i < kRowOctets; i++)
+      if (8 * i < oct) load(part + 8 * i, keep[i]);  // (uniform; past the row's end: zeros)
+#pragma unroll
+    for (int i = 0; i < kRowOctets; i++)
+      if (8 * i < oct) look(keep[i]);
+  } else {
+    for (int o = part; o < oct; o += 8) {
+      load(o, keep[0]);
+      look(keep[0]);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o < 64; o <<= 1) {
+    top = fmaxf(top, __shfl_xor(top, o, kWave));
+    sq += __shfl_xor(sq, o, kWave);
+  }
+  const int ex = row_exp(top), n = log2_norm(sq);
+  if (part == 0 && in) {
+    a.exps[r] = ex;
+    if (!a.per_expert) a.norm[r] = n;
+  }
+  if (a.per_expert) {  // (one atomic a wave where its rows are one expert's: those of an expert queue up)
+    const int64_t first = min(r0 + w * 8, a.rows - 1) / a.per_expert, end = min(r0 + w * 8 + 7, a.rows - 1) / a.per_expert;
+    int big = in ? n : kNoExp;
+    if (first == end) {
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) big = max(big, __shfl_xor(big, o, kWave));
+      if (lane == 0) atomicMax(&a.norm[first], big);
+    } else if (part == 0 && in) {
+      atomicMax(&a.norm[r / a.per_expert], n);
+    }
+  }
+  if (a.blk) {
+    int big_e = from >= 0 && top > 0.f ? -ex : kNoExp, big_n = kNoExp;  // over the wave's 8 rows
+    if (a.weight && from >= 0) {
+      const float wt = finite_abs(a.weight[a.perm[r]]);
+      big_n = wt > 0.f && n > kNoExp ? n + log2_up(wt) : kNoExp;
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      big_e = max(big_e, __shfl_xor(big_e, o, kWave));
+      big_n = max(big_n, __shfl_xor(big_n, o, kWave));
+    }
+    if (lane == 0) {
+      const int e = a.blk[blockIdx.x];
+      if (a.top && big_e > kNoExp) atomicMax(&a.top[e], big_e);
+      if (a.wnorm && big_n > kNoExp) atomicMax(&a.wnorm[e], big_n);
+    }
+  }
+  if (!in) return;
+  const int64_t piece = a.Kp * a.rows;
+  auto store = [&](int o, float (&v)[8]) {
 #pragma unroll
     for (int u = 0; u < 8; u++) v[u] = ldexpf(v[u], ex);
     put_chunk(a.out + (o * a.rows + r) * 8, piece, v);
+  };
+  if constexpr (REGS) {
+#pragma unroll
+    for (int i = 0; i < kRowOctets; i++)
+      if (part + 8 * i < oct) store(part + 8 * i, keep[i]);
+  } else {
+    for (int o = part; o < oct; o += 8) {
+      load(o, keep[0]);
+      store(o, keep[0]);
+    }
   }
 }
 
 // Columns of W[e] [K, C] as operand rows e C + c of [2][Kp / 8][E C][8], their
-// exponents, and each expert's largest column norm.  64 columns a workgroup.
-__global__ __launch_bounds__(256) void cols_kernel(const float* __restrict__ W, _Float16* __restrict__ out,
-                                                   int* __restrict__ exps, int* __restrict__ norm, int64_t K,
-                                                   int64_t Kp, int64_t C, int64_t rows) {
-  __shared__ float st[4][64];
-  __shared__ double sn[4][64];
-  const int t = threadIdx.x, c = t & 63, g = t >> 6;
+// exponents, and each expert's largest column norm.  64 columns a workgroup of 16
+// waves, each the octets w, w + 16, .. of them.  REGS: as above.
+constexpr int kColOctets = 8;
+template <bool REGS>
+__global__ __launch_bounds__(1024) void cols_kernel(const float* __restrict__ W, _Float16* __restrict__ out,
+                                                    int* __restrict__ exps, int* __restrict__ norm, int64_t K,
+                                                    int64_t Kp, int64_t C, int64_t rows) {
+  __shared__ float st[16][64];
+  __shared__ double sn[16][64];
+  const int t = threadIdx.x, c = t & 63;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int64_t col = (int64_t)blockIdx.x * 64 + c, e = blockIdx.y;
   const bool in = col < C;
   const float* __restrict__ p = W + e * K * C + (in ? col : 0);
+  const int oct = (int)(Kp / 8);
   float top = 0.f;
   double sq = 0.;
-#pragma unroll 8
-  for (int64_t k = g; k < K; k += 4) {
-    const float v = finite_abs(p[k * C]);
-    top = fmaxf(top, v);
-    sq += (double)v * v;
+  auto load = [&](int o, float (&v)[8]) {
+#pragma unroll
+    for (int u = 0; u < 8; u++) v[u] = p[(o * 8 + u < K ? o * 8 + u : 0) * C];  // (uniform)
+#pragma unroll
+    for (int u = 0; u < 8; u++) v[u] = o * 8 + u < K ? v[u] : 0.f;
+  };
+  auto look = [&](const float (&v)[8]) {
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const float s = finite_abs(v[u]);
+      top = fmaxf(top, s);
+      sq += (double)s * s;
+    }
+  };
+  float keep[REGS ? kColOctets : 1][8];
+  if constexpr (REGS) {
+#pragma unroll
+    for (int i = 0; i < kColOctets; i++)
+      if (w + 16 * i < oct) load(w + 16 * i, keep[i]);
+#pragma unroll
+    for (int i = 0; i < kColOctets; i++)
+      if (w + 16 * i < oct) look(keep[i]);
+  } else {
+    for (int o = w; o < oct; o += 16) {
+      load(o, keep[0]);
+      look(keep[0]);
+    }
   }
-  st[g][c] = top;
-  sn[g][c] = sq;
+  st[w][c] = top;
+  sn[w][c] = sq;
   __syncthreads();
-  top = fmaxf(fmaxf(st[0][c], st[1][c]), fmaxf(st[2][c], st[3][c]));
+  sq = 0.;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    top = fmaxf(top, st[i][c]);
+    sq += sn[i][c];
+  }
   const int ex = row_exp(top);
-  if (g == 0) {
-    int n = in ? log2_norm(sn[0][c] + sn[1][c] + sn[2][c] + sn[3][c]) : kNoExp;
+  if (w == 0) {
+    int n = in ? log2_norm(sq) : kNoExp;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n = max(n, __shfl_xor(n, o, kWave));
     if (c == 0) atomicMax(&norm[e], n);
@@ -217,15 +279,20 @@ __global__ __launch_bounds__(256) void cols_kernel(const float* __restrict__ W, 
   }
   if (!in) return;
   const int64_t piece = Kp * rows;
-  for (int64_t o = g; o < Kp / 8; o += 4) {
-    float v[8];
+  auto store = [&](int o, float (&v)[8]) {
 #pragma unroll
-    for (int u = 0; u < 8; u++) {
-      const bool ok = o * 8 + u < K;
-      const float f = p[(ok ? o * 8 + u : 0) * C];
-      v[u] = ok ? ldexpf(f, ex) : 0.f;
-    }
+    for (int u = 0; u < 8; u++) v[u] = ldexpf(v[u], ex);
     put_chunk(out + (o * rows + e * C + col) * 8, piece, v);
+  };
+  if constexpr (REGS) {
+#pragma unroll
+    for (int i = 0; i < kColOctets; i++)
+      if (w + 16 * i < oct) store(w + 16 * i, keep[i]);
+  } else {
+    for (int o = w; o < oct; o += 16) {
+      load(o, keep[0]);
+      store(o, keep[0]);
+    }
   }
 }
 
@@ -333,9 +400,9 @@ __device__ __forceinline__ int hidden_seg_exp(const SplitArgs& g, int e) {
 
 template <int MODE>
 __global__ __launch_bounds__(64 * kWaves, 2) void split_kernel(SplitArgs g) {
-  static_assert(kTurnBytes * kWaves <= Tile::kLds, "the transposing tiles fit");
+  static_assert(kTurnBytes * kWaves + 4 * Tile::RA <= Tile::kLds, "the transposing tiles and the exponents fit");
   __shared__ __attribute__((aligned(16))) char smem[Tile::kLds];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 2, wn = wave & 3;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / kWN, wn = wave % kWN;
   const int l32 = lane & 31, kh = lane >> 5;
   int e, mt;
   int64_t n0, nend;       // columns: positions, or kWeight the second matrix's
@@ -401,6 +468,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void split_kernel(SplitArgs g) {
     return;
   } else {
     char* turn = smem + wave * kTurnBytes;
+    int* aexp = reinterpret_cast<int*>(smem + kWaves * kTurnBytes);  // of the tile's rows
+    for (int i = threadIdx.x; i < Tile::RA; i += 64 * kWaves) aexp[i] = g.aexp[arow + min(m0 + i, g.M - 1)];
+    __syncthreads();
     // what a lane knows of its column (position) in block column c
     struct Column {
       int64_t pos;
@@ -440,15 +510,28 @@ __global__ __launch_bounds__(64 * kWaves, 2) void split_kernel(SplitArgs g) {
       const int64_t row0 = mw + r * 32, pos = cl.pos;
       const bool in = pos < nend;
       half4 th[4], tl[4];
+      float pre[4][4];  // the block's pre-activations, all loads in flight at once
+      if constexpr (MODE == kBack) {
+        const float* p = g.pre + (in ? pos : nend - 1) * g.M;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const int64_t k = row0 + 8 * q + 4 * kh;
+          if (g.vec) {
+            const float4 v = *reinterpret_cast<const float4*>(p + min(k, g.M - 4));
+            pre[q][0] = v.x; pre[q][1] = v.y; pre[q][2] = v.z; pre[q][3] = v.w;
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; u++) pre[q][u] = p[min(k + u, g.M - 1)];
+          }
+        }
+      }
 #pragma unroll
       for (int q = 0; q < 4; q++) {
         const int64_t k = row0 + 8 * q + 4 * kh;  // four rows of C: k .. k + 3
         float x[4];
+        const int* ae = aexp + wm * kTM * 32 + r * 32 + 8 * q + 4 * kh;
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-          const int ae = g.aexp[arow + min(k + u, g.M - 1)];
-          x[u] = k + u < g.M ? ldexpf(x16[4 * q + u], -(ae + cl.be)) : 0.f;
-        }
+        for (int u = 0; u < 4; u++) x[u] = k + u < g.M ? ldexpf(x16[4 * q + u], -(ae[u] + cl.be)) : 0.f;
         if constexpr (MODE == kSlots) {
           if (cl.slot < 0) continue;
           float* p = f + (int64_t)cl.slot * g.M + k;
@@ -482,17 +565,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void split_kernel(SplitArgs g) {
               l[u] = ll;
             }
           } else {
-            float up[4] = {0.f, 0.f, 0.f, 0.f};
-            if (in && k < g.M) {
-              const float* p = g.pre + pos * g.M + k;
-              if (g.vec) {
-                const float4 v = *reinterpret_cast<const float4*>(p);
-                up[0] = v.x; up[1] = v.y; up[2] = v.z; up[3] = v.w;
-              } else {
-#pragma unroll
-                for (int u = 0; u < 4; u++) up[u] = k + u < g.M ? p[u] : 0.f;
-              }
-            }
+            const float* up = pre[q];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
               const bool ok = cl.slot >= 0 && k + u < g.M;
@@ -627,10 +700,21 @@ State state_at(Room& r, const MoeShape& m) {
 
 int rows_pass(RowsArgs a, hipStream_t s) {
   const dim3 g((unsigned)ceil_div(a.rows, 32));
-  if (a.K % 4 == 0 && (reinterpret_cast<uintptr_t>(a.src) & 15) == 0)
-    hipLaunchKernelGGL(rows_kernel<true>, g, dim3(256), 0, s, a);
+  const bool vec = a.K % 4 == 0 && (reinterpret_cast<uintptr_t>(a.src) & 15) == 0, regs = a.Kp <= 64 * kRowOctets;
+  if (vec && regs) hipLaunchKernelGGL((rows_kernel<true, true>), g, dim3(256), 0, s, a);
+  else if (vec) hipLaunchKernelGGL((rows_kernel<true, false>), g, dim3(256), 0, s, a);
+  else if (regs) hipLaunchKernelGGL((rows_kernel<false, true>), g, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((rows_kernel<false, false>), g, dim3(256), 0, s, a);
+  NSH_LAUNCHED();
+  return 0;
+}
+int cols_pass(const float* W, _Float16* out, int* exps, int* norm, int64_t K, int64_t Kp, int64_t C, int64_t E,
+              hipStream_t s) {
+  const dim3 g((unsigned)ceil_div(C, 64), (unsigned)E);
+  if (Kp <= 128 * kColOctets)
+    hipLaunchKernelGGL(cols_kernel<true>, g, dim3(1024), 0, s, W, out, exps, norm, K, Kp, C, E * C);
   else
-    hipLaunchKernelGGL(rows_kernel<false>, g, dim3(256), 0, s, a);
+    hipLaunchKernelGGL(cols_kernel<false>, g, dim3(1024), 0, s, W, out, exps, norm, K, Kp, C, E * C);
   NSH_LAUNCHED();
   return 0;
 }
@@ -758,9 +842,7 @@ int launch_experts_split(const float* x, const int32_t* idx, const float* weight
   a.out = xa; a.exps = st.xexp; a.norm = st.xnorm; a.top = st.xtop;
   a.rows = z.np; a.K = m.D; a.Kp = z.Dp;
   if (rows_pass(a, s) != 0) return -1;
-  hipLaunchKernelGGL(cols_kernel, dim3((unsigned)ceil_div(m.H, 64), (unsigned)m.E), dim3(256), 0, s, W1, w1, w1e,
-                     st.w1norm, m.D, z.Dp, m.H, m.E * m.H);
-  NSH_LAUNCHED();
+  if (cols_pass(W1, w1, w1e, st.w1norm, m.D, z.Dp, m.H, m.E, s) != 0) return -1;
   const int64_t entries = ceil_div(z.N, Tile::RB) + m.E;
   SplitArgs g = split_args(m, st, m.H, act);
   g.A = w1; g.arows = m.E * m.H; g.aexp = w1e;
@@ -768,9 +850,7 @@ int launch_experts_split(const float* x, const int32_t* idx, const float* weight
   g.f = pre; g.vec = float4_rows(m.H, pre);
   g.out = ha;
   if (split_product<kHidden>(g, entries, s) != 0) return -1;
-  hipLaunchKernelGGL(cols_kernel, dim3((unsigned)ceil_div(m.D, 64), (unsigned)m.E), dim3(256), 0, s, W2, w2, w2e,
-                     w2e + m.E * m.D, m.H, z.Hp, m.D, m.E * m.D);
-  NSH_LAUNCHED();
+  if (cols_pass(W2, w2, w2e, w2e + m.E * m.D, m.H, z.Hp, m.D, m.E, s) != 0) return -1;
   SplitArgs o = split_args(m, st, m.D, act);
   o.A = w2; o.arows = m.E * m.D; o.aexp = w2e;
   o.B = ha; o.brows = z.np; o.kp = z.Hp;
