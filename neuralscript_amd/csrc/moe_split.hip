@@ -27,6 +27,7 @@
 // x and dy gathered by position, and for the gradient both once more with
 // positions as k.  They are bound by HBM.
 #include <algorithm>
+#include <cstdlib>
 
 #include "common.h"
 #include "kernels.h"
@@ -37,7 +38,9 @@ namespace nship {
 namespace {
 
 // 256 rows x 128 columns, two workgroups on a CU: one's epilogue runs beside the
-// other's products (256 x 256 and one workgroup of eight waves: TODO).
+// other's products.  131072 slots of 64 experts of 1024 x 1024, us, hidden and slots
+// products: 1172, 949 (235 and 290 TFLOP/s); 256 x 256, one workgroup of eight waves
+// on a CU: 1308, 1050.
 constexpr int kTM = 4, kTN = 2, kWM = 2, kWN = 2, kWaves = kWM * kWN;
 using Tile = Split2Tile<kWM, kWN, kTM, kTN, 16>;
 constexpr int kPad = 32;      // positions a segment is padded to
@@ -569,7 +572,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void split_kernel(SplitArgs g) {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
               const bool ok = cl.slot >= 0 && k + u < g.M;
-              const float a = act_apply(up[u], g.act), du = cl.wt * x[u] * act_slope(up[u], g.act), hw = cl.wt * a;
+              float a, slope;
+              act_both(up[u], g.act, a, slope);
+              const float du = cl.wt * x[u] * slope, hw = cl.wt * a;
               cl.dot += ok ? a * x[u] : 0.f;
               _Float16 hh, ll;
               split2_any(ok ? ldexpf(du, cl.oe) : 0.f, hh, ll);
@@ -728,10 +733,21 @@ bool sigmoid_bound(int act) { return act == kActSigmoid; }
 
 }  // namespace
 
+// Both products on pieces cost the layouts of the weights (24 bytes an element,
+// forward) and some 50 us of passes, and save half of the products' time.  Sorted
+// fp32 operands -> this, us, forward and training step: 64 experts of 1024 x 1024,
+// slots an expert 192: 438, 1426 -> 501, 1461; 256: 598, 1879 -> 636, 1827; 384:
+// 808, 2559 -> 740, 2162; 1024: 1835, 5924 -> 1391, 4178.  16 of 512 x 2048, 384:
+// 298, 839 -> 292, 807.  8 of 256 x 256, 1024: 85, 222 -> 133, 357.  Where a size is
+// no multiple of 4 the others read it float by float: 10 of 200 x 333, 96: 118, 282
+// -> 117, 300; 192: 124, 323 -> 121, 317; 1024: 155, 416 -> 138, 392.
+// NSHIP_MOE_SPLIT_MIN (a testing knob): the least slots an expert, of any size.
 bool split_takes(const MoeShape& m) {
   if (m.D <= 128 || m.H <= 128) return false;
-  const int64_t per = (m.D % 4 || m.H % 4) ? 32 : 384;
-  return m.T * m.K >= per * m.E;
+  const int64_t N = m.T * m.K;
+  if (const char* knob = getenv("NSHIP_MOE_SPLIT_MIN")) return N >= std::max<int64_t>(1, atoll(knob)) * m.E;
+  const bool odd = m.D % 4 || m.H % 4;
+  return N >= (odd ? 192 : 288) * m.E && (double)N * m.D * m.H >= (odd ? 0x1p28 : 6 * 0x1p30);
 }
 
 static size_t split_forward(const MoeShape& m, Room& r, bool state, State* st, int** count, _Float16** xa,

@@ -631,9 +631,11 @@ __global__ __launch_bounds__(256) void bwd_rows_kernel(const float* __restrict__
   const float w = weight[slot];
   float dot = 0.f;
   for (int a = lane; a < H; a += 64) {
-    const float u = pre[pos * H + a], d = dh[pos * H + a], h = act_apply(u, act);
+    const float d = dh[pos * H + a];
+    float h, slope;
+    act_both(pre[pos * H + a], act, h, slope);
     dot += h * d;
-    dh[pos * H + a] = w * d * act_slope(u, act);
+    dh[pos * H + a] = w * d * slope;
     hw[pos * H + a] = w * h;
   }
   dot = wave_sum(dot);

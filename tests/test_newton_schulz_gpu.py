@@ -210,11 +210,15 @@ def test_a_sparse_layers_training_step():
             assert d <= a.LR * np.sqrt(min(D, H)) * 485 * 1e-5, (k, e, d)
 
 
-def test_a_training_step_captured_and_replayed():
+@pytest.mark.parametrize("pieces", [False, True])
+def test_a_training_step_captured_and_replayed(pieces, monkeypatch):
     """Two layers of different sizes as two graphs, replayed in turn with eager
     steps of a third between them: every replay gives the eager steps' bits."""
     stream = so.new_stream()
     sizes = [(96, 2, 64, 96, 5), (12, 3, 36, 20, 4)]
+    if pieces:
+        monkeypatch.setenv("NSHIP_MOE_SPLIT_MIN", "16")
+        sizes = [(200, 2, 136, 260, 5), (150, 3, 200, 140, 4)]
     eager = []
     for i, s in enumerate(sizes):
         a = Layer(*s, i)
