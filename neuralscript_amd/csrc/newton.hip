@@ -34,7 +34,7 @@ namespace {
 
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
 constexpr double kNsEps = 1e-7;
-constexpr int kNormParts = 64;  // partial sums of a matrix's norm
+constexpr int kNormParts = 256;  // partial sums of a matrix's norm
 // the operands' powers of two: X and S below 2 x 2^15 = fp16's range, P below 4 x 2^14
 constexpr float kUpX = 0x1p15f, kUpS = 0x1p15f, kUpP = 0x1p14f;
 
@@ -238,6 +238,7 @@ __global__ __launch_bounds__(512) void ns_few_kernel(NsArgs g) {
         b[u][0] = pb[o * g.rb];
         b[u][1] = pb[o * g.rb + lb];
       }
+      __builtin_amdgcn_sched_barrier(0);  // (all loads first)
 #pragma unroll
       for (int u = 0; u < CNT; u++) {
         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][1], b[u][0], acc, 0, 0, 0);
@@ -272,6 +273,98 @@ __global__ __launch_bounds__(512) void ns_few_kernel(NsArgs g) {
   ns_epilogue<MODE, 1, 1>(g, one, reinterpret_cast<char*>(part), mat, mw, nw, l32, kh, kSym && tm == tn);
 }
 
+// ... and between the two: 64 x 64 outputs a workgroup, each of the eight waves
+// with the whole tile over its share of K (half of the loads a product that 32 x
+// 32 outputs take), the eight sums met in LDS, where wave (i, j) of the first four
+// takes its block's.
+constexpr int kMidU = 3;
+template <int MODE>
+__global__ __launch_bounds__(512) void ns_mid_kernel(NsArgs g) {
+  constexpr bool kSym = MODE == kGram || MODE == kPoly;
+  __shared__ __attribute__((aligned(16))) float part[4][4][1024];  // [wave pair][block]
+  const int t = threadIdx.x, lane = t & 63, l32 = lane & 31, kh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int L = split2_xcd_linear(blockIdx.x, g.tiles * g.n);
+  const int mat = L / g.tiles;
+  int tm, tn;
+  ns_tile<kSym>(L % g.tiles, g.tiles_n, tm, tn);
+  const int64_t mw = (int64_t)tm * 64, nw = (int64_t)tn * 64;
+  floatx16 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) acc[i][j][v] = 0.f;
+  {
+    const half8 *pa[2], *pb[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      pa[i] = reinterpret_cast<const half8*>(g.A + mat * g.sA) + kh * g.ra + min(mw + 32 * i + l32, g.ra - 1);
+      pb[i] = reinterpret_cast<const half8*>(g.B + mat * g.sB) + kh * g.rb + min(nw + 32 * i + l32, g.rb - 1);
+    }
+    const int64_t la = g.k / 8 * g.ra, lb = g.k / 8 * g.rb;  // to the other piece
+    const int all = (int)(g.k / 16);
+    auto steps = [&](int s0, auto count) {
+      constexpr int CNT = decltype(count)::value;
+      half8 a[CNT][2][2], b[CNT][2][2];
+#pragma unroll
+      for (int u = 0; u < CNT; u++) {
+        const int64_t o = 2 * ((int64_t)s0 + 8 * u);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          a[u][i][0] = pa[i][o * g.ra];
+          a[u][i][1] = pa[i][o * g.ra + la];
+          b[u][i][0] = pb[i][o * g.rb];
+          b[u][i][1] = pb[i][o * g.rb + lb];
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < CNT; u++)
+#pragma unroll
+        for (int q = 0; q < 3; q++)  // l h, h l, h h
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][i][q == 0], b[u][j][q == 1], acc[i][j], 0, 0, 0);
+    };
+    int s = wave;
+    for (; s + 8 * (kMidU - 1) < all; s += 8 * kMidU) steps(s, std::integral_constant<int, kMidU>{});
+    if (s + 8 < all) {
+      steps(s, std::integral_constant<int, 2>{});
+      s += 16;
+    }
+    if (s < all) steps(s, std::integral_constant<int, 1>{});
+  }
+  if (wave >= 4) {
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) part[wave - 4][q][v * 64 + lane] = acc[q >> 1][q & 1][v];
+  }
+  __syncthreads();
+  if (wave >= 4) return;
+  // (waves 4 .. 7 are gone: a barrier counts the four that are left)
+#pragma unroll
+  for (int q = 0; q < 4; q++)
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+      acc[q >> 1][q & 1][v] += part[wave][q][v * 64 + lane];
+      part[wave][q][v * 64 + lane] = acc[q >> 1][q & 1][v];
+    }
+  __syncthreads();
+  floatx16 one[1][1];
+#pragma unroll
+  for (int v = 0; v < 16; v++)
+    one[0][0][v] = (part[0][wave][v * 64 + lane] + part[1][wave][v * 64 + lane]) +
+                   (part[2][wave][v * 64 + lane] + part[3][wave][v * 64 + lane]);
+  __syncthreads();
+  ns_epilogue<MODE, 1, 1>(g, one, reinterpret_cast<char*>(part) + wave * kTurnBytes, mat, mw + (wave >> 1) * 32,
+                          nw + (wave & 1) * 32, l32, kh, kSym && tm == tn);
+}
+
 __device__ __forceinline__ float update_of(float g, float m, float mu, int nesterov) {
   return nesterov ? g + mu * m : m;
 }
@@ -283,14 +376,26 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const float* __restrict__ 
   __shared__ double red[4];
   const int64_t base = (int64_t)blockIdx.y * elems;
   double sum = 0.;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elems; i += (int64_t)gridDim.x * 256) {
-    float u = g[base + i];
-    if (m) {
-      const float mm = mu * m[base + i] + u;
-      m[base + i] = mm;
-      u = update_of(u, mm, mu, nesterov);
+  const int64_t step = (int64_t)gridDim.x * 256;
+  for (int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x; i0 < elems; i0 += 8 * step) {
+    float u[8], mm[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int64_t i = min(i0 + j * step, elems - 1);
+      u[j] = g[base + i];
+      if (m) mm[j] = m[base + i];
     }
-    sum += (double)u * u;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int64_t i = i0 + j * step;
+      if (i >= elems) break;
+      if (m) {
+        mm[j] = mu * mm[j] + u[j];
+        m[base + i] = mm[j];
+        u[j] = update_of(u[j], mm[j], mu, nesterov);
+      }
+      sum += (double)u[j] * u[j];
+    }
   }
   sum = wave_sum(sum);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
@@ -298,14 +403,21 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const float* __restrict__ 
   if (threadIdx.x == 0) part[(int64_t)blockIdx.y * kNormParts + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
+// e0: 2^e0 |X0| in (1/2, 1].  (|X0| is at least 1e-38.)
+__device__ __forceinline__ int ns_exponent(double x0) { return x0 > 0. ? max(0, min(126, ilogb(1. / x0))) : 0; }
+
 // 1 / (|u|_F + 1e-7) from the partial sums; NaN where the norm is not finite,
 // so that the whole matrix is.
 __device__ __forceinline__ double ns_scale(const double* __restrict__ part, int parts, int* ex = nullptr) {
-  const int lane = threadIdx.x & 63;  // (parts <= 64)
-  const double sq = wave_sum(lane < parts ? part[lane] : 0.);
+  const int lane = threadIdx.x & 63;
+  double x[kNormParts / 64], some = 0.;
+#pragma unroll
+  for (int i = 0; i < kNormParts / 64; i++) x[i] = part[min(lane + 64 * i, parts - 1)];
+#pragma unroll
+  for (int i = 0; i < kNormParts / 64; i++) some += lane + 64 * i < parts ? x[i] : 0.;
+  const double sq = wave_sum(some);
   const double norm = sqrt(sq), by = sq < __builtin_inf() ? 1. / (norm + kNsEps) : __builtin_nan("");
-  // 2^ex |X0| in (1/2, 1]: |X0| is at least 1e-38, since no smaller float has a square here
-  if (ex) *ex = norm * by > 0. ? max(0, min(126, ilogb(1. / (norm * by)))) : 0;
+  if (ex) *ex = ns_exponent(norm * by);
   return by;
 }
 
@@ -327,26 +439,31 @@ struct NsStart {
 __global__ __launch_bounds__(256) void ns_start_kernel(NsStart a) {
   __shared__ float x[64][65];  // [i][j] of X
   const int64_t elems = a.r * a.c, base = (int64_t)blockIdx.y * elems;
-  int ex;
-  const double by = ns_scale(a.part + (int64_t)blockIdx.y * kNormParts, a.parts, &ex);
-  const double up = ldexp(by * kUpX, ex);
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.ex[blockIdx.y] = ex;
   const int64_t i0 = (int64_t)(blockIdx.x / a.tiles_n) * 64, j0 = (int64_t)(blockIdx.x % a.tiles_n) * 64;
   const int t = threadIdx.x, lo = t & 63, hi = t >> 6;
   const bool tall = a.r > a.c;
+  float u[16];
 #pragma unroll
   for (int q = 0; q < 16; q++) {
     const int h = hi + 4 * q;  // (lanes run along g's rows)
     const int64_t i = i0 + (tall ? lo : h), j = j0 + (tall ? h : lo);
-    float u = 0.f;
+    u[q] = 0.f;
     if (i < a.M && j < a.N) {
       const int64_t at = base + (tall ? j * a.c + i : i * a.c + j);
-      u = a.g[at];
-      if (a.m) u = update_of(u, a.m[at], a.mu, a.nesterov);
-      u = (float)(u * up);
+      u[q] = a.g[at];
+      if (a.m) u[q] = update_of(u[q], a.m[at], a.mu, a.nesterov);
     }
-    if (tall) x[lo][h] = u;
-    else x[h][lo] = u;
+  }
+  int ex;
+  const double by = ns_scale(a.part + (int64_t)blockIdx.y * kNormParts, a.parts, &ex);
+  const double up = ldexp(by * kUpX, ex);
+  if (blockIdx.x == 0 && t == 0) a.ex[blockIdx.y] = ex;
+#pragma unroll
+  for (int q = 0; q < 16; q++) {
+    const int h = hi + 4 * q;
+    const float v = (float)(u[q] * up);
+    if (tall) x[lo][h] = v;
+    else x[h][lo] = v;
   }
   __syncthreads();
   const int64_t pg = a.np * a.M, pu = a.mp * a.N;
@@ -400,99 +517,149 @@ __global__ __launch_bounds__(256) void ns_normalise_kernel(const float* g, const
 }
 
 // A small matrix's whole orthogonalisation by one workgroup of 16 waves: X both
-// ways and S (then P in its place) in LDS as the products above hold them,
-// padded so (8 m N + 4 m^2 bytes: up to 64 x 256).  A step is three products
-// of a few 16 x 16 blocks a wave with a barrier between (blocks of 32 x 32 leave
-// most waves without one).  Bound by the latency of LDS reads and MFMAs.
+// ways and S (then P in its place) in LDS as the products above hold them, padded
+// to 32 and with a row more between octets (the epilogues' stores along k then
+// spread over the banks): up to 64 x 256.  A step is three products with a barrier
+// between: S and P in 16 x 16 blocks (of 32 x 32 most waves would have none), X in
+// 32 x 32 ones (half of the LDS reads).  Bound by LDS traffic and the waves'
+// latency: 8 of 64 x 256 in 5 steps: see launch_newton_schulz.
 constexpr int kNsLds = 163840;
 struct NsFused {
   const float* g;
   float* m;
   float mu;
   int nesterov, r, c, M, N, mp, np, steps;
+  int vec;  // rows of g and m are read as float4
   float* f;
   float le, decay;
   int weights;
 };
+// LDS bytes of X (both ways) and S.
+__host__ __device__ constexpr int64_t ns_fused_bytes(int64_t mp, int64_t np) {
+  return 4 * (np * (mp + 1) + mp * (np + 1) + mp * (mp + 1));
+}
 __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
   extern __shared__ __attribute__((aligned(16))) char ns_lds[];
   __shared__ double red[16];
-  constexpr int kW = 16, kSymBlocks = 2, kBlocks = 5;  // waves, blocks of S and of X a wave (ns_fused_fits)
-  const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, kq = lane >> 4;
+  constexpr int kW = 16, kSymBlocks = 2, kBlocks = 2;  // waves, blocks of S and of X a wave (ns_fused_fits)
+  const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int mp = a.mp, np = a.np, mb = mp / 16, nb = np / 16;
-  _Float16* gram = reinterpret_cast<_Float16*>(ns_lds);  // [2][np / 8][mp][8]
-  _Float16* upd = gram + 2 * np * mp;                    // [2][mp / 8][np][8]
-  _Float16* sym = upd + 2 * np * mp;                     // [2][mp / 8][mp][8]
-  const int px = np * mp, ps = mp * mp;                  // to the other piece
+  const int mp = a.mp, np = a.np;
+  int rm = mp + 1, rn = np + 1;  // rows between octets
+  const int pg = np * rm, pu = mp * rn, ps = mp * rm;        // to the other piece, halves
+  _Float16* gram = reinterpret_cast<_Float16*>(ns_lds);  // [2][np / 8][rm][8]
+  _Float16* upd = gram + 2 * pg;                         // [2][mp / 8][rn][8]
+  _Float16* sym = upd + 2 * pu;                          // [2][mp / 8][rm][8]
   const int elems = a.r * a.c;
   const int64_t base = (int64_t)blockIdx.x * elems;
   const float* __restrict__ g = a.g + base;
   float* __restrict__ m = a.m ? a.m + base : nullptr;
   const bool tall = a.r > a.c;
   double sq = 0.;
-#pragma unroll 4
-  for (int i = t; i < elems; i += 64 * kW) {
-    float u = g[i];
-    if (m) {
-      const float mm = a.mu * m[i] + u;
-      m[i] = mm;
-      u = update_of(u, mm, a.mu, a.nesterov);
+  for (int i0 = t; i0 < elems; i0 += 8 * 64 * kW) {
+    float u[8], mm[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int i = min(i0 + j * 64 * kW, elems - 1);
+      u[j] = g[i];
+      if (m) mm[j] = m[i];
     }
-    sq += (double)u * u;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int i = i0 + j * 64 * kW;
+      if (i >= elems) break;
+      if (m) {
+        mm[j] = a.mu * mm[j] + u[j];
+        m[i] = mm[j];
+        u[j] = update_of(u[j], mm[j], a.mu, a.nesterov);
+      }
+      sq += (double)u[j] * u[j];
+    }
   }
   sq = wave_sum(sq);
   if (lane == 0) red[wave] = sq;
-  for (int i = t; i < px / 2; i += 64 * kW) reinterpret_cast<uintx4*>(gram)[i] = uintx4{0u, 0u, 0u, 0u};  // (both of X)
-  __syncthreads();
-  int e0;
-  const double up = ldexp(ns_scale(red, kW, &e0) * kUpX, e0);
-  // a chunk at a time: eight k of a row, of X (i, j) at i * c + j or, tall, j * c + i
-  const int si1 = tall ? 1 : a.c, sj1 = tall ? a.c : 1;
-  auto chunks = [&](_Float16* to, int rows, int nrows, int ks, int row_step, int k_step) {
-    // (rows of the operand in consecutive lanes; octets past the end stay zero)
-    for (int c = t; c < ((ks + 7) >> 3) * nrows; c += 64 * kW) {
-      const int o = c / nrows, row = c - o * nrows;
-      half8 h, l;
+  for (int i = t; i < (pg + pu) / 4; i += 64 * kW) reinterpret_cast<uintx4*>(gram)[i] = uintx4{0u, 0u, 0u, 0u};
+  __syncthreads();  // (m is written: other threads read it below)
+  sq = wave_sum(lane < kW ? red[lane] : 0.);
+  const double norm = sqrt(sq), by = sq < __builtin_inf() ? 1. / (norm + kNsEps) : __builtin_nan("");
+  const int e0 = ns_exponent(norm * by);
+  const double up = ldexp(by * kUpX, e0);
+  // X into an operand a chunk at a time: eight k of a row
+  auto chunk = [&](_Float16* to, int rows, int piece, int ks, int row_step, int k_step, int row, int o) {
+    float v[8];
+    if (a.vec && k_step == 1) {  // (uniform; rows of a multiple of 4)
+#pragma unroll
+      for (int u = 0; u < 8; u += 4) {
+        const int at = row * row_step + min(8 * o + u, ks - 4);
+        float4 f = *reinterpret_cast<const float4*>(g + at);
+        if (m) {
+          const float4 h = *reinterpret_cast<const float4*>(m + at);
+          f = make_float4(update_of(f.x, h.x, a.mu, a.nesterov), update_of(f.y, h.y, a.mu, a.nesterov),
+                          update_of(f.z, h.z, a.mu, a.nesterov), update_of(f.w, h.w, a.mu, a.nesterov));
+        }
+        v[u] = f.x; v[u + 1] = f.y; v[u + 2] = f.z; v[u + 3] = f.w;
+      }
+    } else {
 #pragma unroll
       for (int u = 0; u < 8; u++) {
-        const int k = 8 * o + u;
-        const int at = row * row_step + min(k, ks - 1) * k_step;
-        float v = g[at];
-        if (m) v = update_of(v, m[at], a.mu, a.nesterov);
-        v = k < ks ? (float)(v * up) : 0.f;
-        _Float16 hh, ll;
-        split2(v, hh, ll);
-        h[u] = hh;
-        l[u] = ll;
+        const int at = row * row_step + min(8 * o + u, ks - 1) * k_step;
+        v[u] = g[at];
+        if (m) v[u] = update_of(v[u], m[at], a.mu, a.nesterov);
       }
-      _Float16* p = to + (o * rows + row) * 8;
-      *reinterpret_cast<half8*>(p) = h;
-      *reinterpret_cast<half8*>(p + px) = l;
+    }
+    half8 h, l;
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      _Float16 hh, ll;
+      split2(8 * o + u < ks ? (float)(v[u] * up) : 0.f, hh, ll);
+      h[u] = hh;
+      l[u] = ll;
+    }
+    _Float16* p = to + (o * rows + row) * 8;
+    *reinterpret_cast<half8*>(p) = h;
+    *reinterpret_cast<half8*>(p + piece) = l;
+  };
+  // a wave takes 64 rows of an octet where rows lie next to each other in g, else 8
+  // rows of 8 octets
+  auto chunks = [&](_Float16* to, int rows, int piece, int nrows, int ks, int row_step, int k_step) {
+    const int octs = (ks + 7) >> 3;
+    if (k_step == 1) {
+      const int across = (octs + 7) >> 3;
+      for (int b = wave; b < across * ((nrows + 7) >> 3); b += kW) {
+        const int o = b % across * 8 + (lane >> 3), row = b / across * 8 + (lane & 7);
+        if (o < octs && row < nrows) chunk(to, rows, piece, ks, row_step, k_step, row, o);
+      }
+    } else {
+      const int across = (nrows + 63) >> 6;
+      for (int b = wave; b < across * octs; b += kW) {
+        const int row = b % across * 64 + lane;
+        if (row < nrows) chunk(to, rows, piece, ks, row_step, k_step, row, b / across);
+      }
     }
   };
-  chunks(gram, mp, a.M, a.N, si1, sj1);
-  chunks(upd, np, a.N, a.M, sj1, si1);
+  const int si1 = tall ? 1 : a.c, sj1 = tall ? a.c : 1;  // X (i, j) is g[i si1 + j sj1]
+  chunks(gram, rm, pg, a.M, a.N, si1, sj1);
+  chunks(upd, rn, pu, a.N, a.M, sj1, si1);
   __syncthreads();
-  // 16 x 16 block (bi, bj) of A B^T over `steps` of 32: lane (l16, kq) holds
-  // octet kq of a step, then column l16 of rows 4 kq ..
-  auto block = [&](const _Float16* A, int ra, int la, int bi, const _Float16* B, int rb, int lb, int bj, int steps) {
-    const half8* pa = reinterpret_cast<const half8*>(A) + kq * ra + bi * 16 + l16;
-    const half8* pb = reinterpret_cast<const half8*>(B) + kq * rb + bj * 16 + l16;
-    la /= 8;
-    lb /= 8;
+  // 16 x 16 block (bi, bj) of A A^T, A of rows rm, over `steps` of 32: lane (l16, kq)
+  // holds octet kq of a step, then column l16 of rows 4 kq ..
+  int l16 = lane & 15, kq = lane >> 4;
+  auto block16 = [&](const _Float16* A, int piece, int bi, int bj, int steps) {
+    const half8* pa = reinterpret_cast<const half8*>(A) + kq * rm + bi * 16 + l16;
+    const half8* pb = reinterpret_cast<const half8*>(A) + kq * rm + bj * 16 + l16;
+    piece /= 8;
     floatx4 hi = {0.f, 0.f, 0.f, 0.f}, lo = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
+#pragma unroll 4
     for (int s = 0; s < steps; s++) {
-      const half8 a0 = pa[4 * s * ra], a1 = pa[4 * s * ra + la], b0 = pb[4 * s * rb], b1 = pb[4 * s * rb + lb];
+      const half8 a0 = pa[4 * s * rm], a1 = pa[4 * s * rm + piece], b0 = pb[4 * s * rm], b1 = pb[4 * s * rm + piece];
       hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b0, hi, 0, 0, 0);
       lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, b0, lo, 0, 0, 0);
       lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b1, lo, 0, 0, 0);
     }
     return hi + lo;
   };
-  // a block's values as operand [k = row][col] of rows r and, other not null, as [k = col][row] of rows ro
-  auto put = [&](const floatx4& x, int bi, int bj, _Float16* to, int r, int piece, _Float16* other, int ro) {
+  // its values into S's or P's operand, both ways unless on the diagonal
+  auto put16 = [&](const floatx4& x, int bi, int bj) {
     const int col = bj * 16 + l16, row = bi * 16 + 4 * kq;
     half4 h, l;
 #pragma unroll
@@ -501,81 +668,115 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
       split2(x[u], hh, ll);
       h[u] = hh;
       l[u] = ll;
-      if (other) {
-        _Float16* p = other + ((col >> 3) * ro + row + u) * 8 + (col & 7);
+      if (bi != bj) {
+        _Float16* p = sym + ((col >> 3) * rm + row + u) * 8 + (col & 7);
         p[0] = hh;
-        p[piece] = ll;
+        p[ps] = ll;
       }
     }
-    _Float16* p = to + ((row >> 3) * r + col) * 8 + (row & 7);
+    _Float16* p = sym + ((row >> 3) * rm + col) * 8 + (row & 7);
     *reinterpret_cast<half4*>(p) = h;
-    *reinterpret_cast<half4*>(p + piece) = l;
+    *reinterpret_cast<half4*>(p + ps) = l;
   };
-  const int tri = mb * (mb + 1) / 2;
+  const int mb = mp / 16, tri = mb * (mb + 1) / 2;
   int si[kSymBlocks], sj[kSymBlocks];
 #pragma unroll
   for (int q = 0; q < kSymBlocks; q++) ns_tile<true>(wave + kW * q, 0, si[q], sj[q]);
+  const int xb = mp / 32, nb = np / 32;
+  int l32 = lane & 31, kh = lane >> 5;
   for (int step = 0; step < a.steps; step++) {
+    // (keeps the compiler from holding every address of a step in registers)
+    asm volatile("" : "+s"(rm), "+s"(rn), "+v"(l16), "+v"(kq), "+v"(l32), "+v"(kh));
     const int ex = max(0, e0 - 2 * step);
-    floatx4 S[kSymBlocks], P[kSymBlocks];
+    floatx4 S[kSymBlocks];
 #pragma unroll
-    for (int q = 0; q < kSymBlocks; q++) {
-      if (wave + kW * q >= tri) break;
-      S[q] = block(gram, mp, px, si[q], gram, mp, px, sj[q], np / 32);
+    for (int q = 0; q < kSymBlocks; q++)
+      if (wave + kW * q < tri) {
+        __builtin_amdgcn_sched_barrier(0);  // (a block at a time: registers)
+        S[q] = block16(gram, pg, si[q], sj[q], np / 32);
 #pragma unroll
-      for (int v = 0; v < 4; v++) {
-        // (as P's square sees it: a rounding of S in one term alone would reach P four times as large)
-        _Float16 h, l;
-        split2(S[q][v] * (kUpS / (kUpX * kUpX)), h, l);
-        S[q][v] = (float)h + (float)l;
+        for (int v = 0; v < 4; v++) {
+          // (as P's square sees it: a rounding of S in one term alone would reach P four times as large)
+          _Float16 h, l;
+          split2(S[q][v] * (kUpS / (kUpX * kUpX)), h, l);
+          S[q][v] = (float)h + (float)l;
+        }
+        put16(S[q], si[q], sj[q]);
       }
-      put(S[q], si[q], sj[q], sym, mp, ps, si[q] == sj[q] ? nullptr : sym, mp);
-    }
     __syncthreads();
     const float bs = ldexpf(kNsB * kUpP / kUpS, -2 * ex), bss = ldexpf(kNsC * kUpP / (kUpS * kUpS), -4 * ex);
 #pragma unroll
-    for (int q = 0; q < kSymBlocks; q++) {
-      if (wave + kW * q >= tri) break;
-      P[q] = block(sym, mp, ps, si[q], sym, mp, ps, sj[q], mp / 32);
-      const int col = sj[q] * 16 + l16, row = si[q] * 16 + 4 * kq;
+    for (int q = 0; q < kSymBlocks; q++)
+      if (wave + kW * q < tri) {
+        __builtin_amdgcn_sched_barrier(0);
+        const floatx4 x = block16(sym, ps, si[q], sj[q], mp / 32);
+        const int col = sj[q] * 16 + l16, row = si[q] * 16 + 4 * kq;
 #pragma unroll
-      for (int v = 0; v < 4; v++)
-        P[q][v] = P[q][v] * bss + (row + v == col && col < a.M ? kNsA * kUpP : 0.f) + bs * S[q][v];
-    }
+        for (int v = 0; v < 4; v++)
+          S[q][v] = x[v] * bss + (row + v == col && col < a.M ? kNsA * kUpP : 0.f) + bs * S[q][v];
+      }
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < kSymBlocks; q++) {
-      if (wave + kW * q >= tri) break;
-      put(P[q], si[q], sj[q], sym, mp, ps, si[q] == sj[q] ? nullptr : sym, mp);
-    }
+    for (int q = 0; q < kSymBlocks; q++)
+      if (wave + kW * q < tri) put16(S[q], si[q], sj[q]);
     __syncthreads();
-    floatx4 x[kBlocks];
+    // X: 32 x 32 block (b / nb, b % nb) of P X over the 16-steps of m
+    floatx16 x[kBlocks];
 #pragma unroll
     for (int q = 0; q < kBlocks; q++) {
       const int b = wave + kW * q;
-      if (b >= mb * nb) break;
-      x[q] = block(sym, mp, ps, b / nb, upd, np, px, b % nb, mp / 32);
+      if (b < xb * nb) {
+        __builtin_amdgcn_sched_barrier(0);
+        const half8* pa = reinterpret_cast<const half8*>(sym) + kh * rm + b / nb * 32 + l32;
+        const half8* pb = reinterpret_cast<const half8*>(upd) + kh * rn + b % nb * 32 + l32;
+#pragma unroll
+        for (int v = 0; v < 16; v++) x[q][v] = 0.f;
+#pragma unroll 4
+        for (int s = 0; s < mp / 16; s++) {
+          const half8 a0 = pa[2 * s * rm], a1 = pa[2 * s * rm + ps / 8], b0 = pb[2 * s * rn], b1 = pb[2 * s * rn + pu / 8];
+          x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b0, x[q], 0, 0, 0);
+          x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b1, x[q], 0, 0, 0);
+          x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b0, x[q], 0, 0, 0);
+        }
+      }
     }
     const bool last = step + 1 == a.steps;
-    const float by = last ? ldexpf(1.f / (kUpX * kUpP), -ex) : ldexpf(1.f / kUpP, max(0, ex - 2) - ex);
+    const float xs = last ? ldexpf(1.f / (kUpX * kUpP), -ex) : ldexpf(1.f / kUpP, max(0, ex - 2) - ex);
     if (!last) __syncthreads();
 #pragma unroll
     for (int q = 0; q < kBlocks; q++) {
       const int b = wave + kW * q;
-      if (b >= mb * nb) break;
-      const int bi = b / nb, bj = b % nb;
-      x[q] *= by;
-      if (!last) {
-        put(x[q], bi, bj, upd, np, px, gram, mp);
+      if (b >= xb * nb) continue;
+      __builtin_amdgcn_sched_barrier(0);
+      const int row0 = b / nb * 32 + 4 * kh, col = b % nb * 32 + l32;
+      if (last) {
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+          const int i = row0 + 8 * (v >> 2) + (v & 3);
+          if (i >= a.M || col >= a.N) continue;
+          float* p = a.f + base + (tall ? col * a.c + i : i * a.c + col);
+          const float y = x[q][v] * xs;
+          *p = a.weights ? *p - a.le * y - a.decay * *p : y;
+        }
         continue;
       }
-      const int j = bj * 16 + l16;
 #pragma unroll
-      for (int v = 0; v < 4; v++) {
-        const int i = bi * 16 + 4 * kq + v;
-        if (i >= a.M || j >= a.N) continue;
-        float* p = a.f + base + (tall ? j * a.c + i : i * a.c + j);
-        *p = a.weights ? *p - a.le * x[q][v] - a.decay * *p : x[q][v];
+      for (int w = 0; w < 4; w++) {
+        __builtin_amdgcn_sched_barrier(0);
+        half4 h, l;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          _Float16 hh, ll;
+          split2(x[q][4 * w + u] * xs, hh, ll);
+          h[u] = hh;
+          l[u] = ll;
+          _Float16* p = gram + ((col >> 3) * rm + row0 + 8 * w + u) * 8 + (col & 7);
+          p[0] = hh;
+          p[pg] = ll;
+        }
+        _Float16* p = upd + ((row0 + 8 * w) / 8 * rn + col) * 8 + (row0 & 7);
+        *reinterpret_cast<half4*>(p) = h;
+        *reinterpret_cast<half4*>(p + pu) = l;
       }
     }
     if (!last) __syncthreads();
@@ -583,10 +784,10 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
 }
 
 // Whether a matrix fits ns_fused_kernel: its LDS, and its waves' blocks (which the LDS bounds: m is at
-// most 96, 21 blocks of S on 16 waves, and m N at most 20480, 80 blocks of X).
+// most 96, 21 blocks of S on 16 waves, and m N at most 20480, 20 blocks of X).
 bool ns_fused_fits(int64_t m, int64_t N) {
   const int64_t mp = (m + 31) / 32 * 32, np = (N + 31) / 32 * 32;
-  return np <= 4096 && 8 * mp * np + 4 * mp * mp + 128 <= kNsLds;
+  return np <= 4096 && ns_fused_bytes(mp, np) + 128 <= kNsLds;
 }
 
 constexpr int64_t round64(int64_t n) { return (n + 63) / 64 * 64; }
@@ -614,14 +815,23 @@ int launch_product(NsArgs& g, hipStream_t s) {
     g.tiles = (int)t;
     return t * g.n;
   };
-  if (tiles(256, 256) >= 256)
-    hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 4, 4, 2, 16>), dim3((unsigned)(g.tiles * (int64_t)g.n)), dim3(512), 0, s, g);
-  else if (tiles(128, 128) >= 256)
-    hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 2, 2, 2, 32>), dim3((unsigned)(g.tiles * (int64_t)g.n)), dim3(256), 0, s, g);
-  else {
-    tiles(32, 32);
-    hipLaunchKernelGGL((ns_few_kernel<MODE>), dim3((unsigned)(g.tiles * (int64_t)g.n)), dim3(512), 0, s, g);
-  }
+  // Estimated us of each kernel from its workgroups and K, as measured on 512 x
+  // 512, 4 of 512 x 512, 512 x 2048, 8192 x 512, 2000 x 1500, 8 and 64 of 1024 x
+  // 1024: 32 x 32 outputs a workgroup 4 + 0.0031 K, or 2.2e-5 K each once they fill
+  // the chip; 64 x 64 6 + 0.0075 K, or 6.5e-5 K; 128 x 128 9 + 0.0215 K on a CU by
+  // itself, 1.2 times as much for each of several; 256 x 256 8 + 0.095 K.
+  const double k = (double)g.k;
+  const double t32 = (double)tiles(32, 32), t64 = (double)tiles(64, 64);
+  const int64_t n128 = ceil_div(tiles(128, 128), 256), n256 = ceil_div(tiles(256, 256), 256);
+  const double us[4] = {std::max(4 + 0.0031 * k, 3 + 2.2e-5 * k * t32), std::max(6 + 0.0075 * k, 3 + 6.5e-5 * k * t64),
+                        9 + 0.0215 * k * (n128 == 1 ? 1. : 1.2 * n128), 8 + 0.095 * k * n256};
+  const int64_t side[4] = {32, 64, 128, 256};
+  const int use = (int)(std::min_element(us, us + 4) - us);
+  const dim3 grid((unsigned)tiles(side[use], side[use]));
+  if (use == 0) hipLaunchKernelGGL((ns_few_kernel<MODE>), grid, dim3(512), 0, s, g);
+  else if (use == 1) hipLaunchKernelGGL((ns_mid_kernel<MODE>), grid, dim3(512), 0, s, g);
+  else if (use == 2) hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 2, 2, 2, 32>), grid, dim3(256), 0, s, g);
+  else hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 4, 4, 2, 16>), grid, dim3(512), 0, s, g);
   NSH_LAUNCHED();
   return 0;
 }
@@ -646,7 +856,7 @@ int launch_newton_schulz(const float* g, float* q, const MuonNs* step, int64_t n
   _Float16* upd2 = upd + n * z.upd;
   _Float16* S = upd2 + n * z.upd;
   _Float16* P = S + n * z.sym;
-  const int parts = (int)std::min<int64_t>(kNormParts, ceil_div(elems, 1024));
+  const int parts = (int)std::min<int64_t>(kNormParts, ceil_div(elems, 2048));
   float* mom = step ? step->m : nullptr;
   const float mu = step ? step->mu : 0.f;
   const int nesterov = step ? step->nesterov : 0;
@@ -661,7 +871,8 @@ int launch_newton_schulz(const float* g, float* q, const MuonNs* step, int64_t n
     f.weights = step != nullptr;
     f.le = step ? step->le : 0.f;
     f.decay = step ? step->decay : 0.f;
-    const unsigned lds = (unsigned)(8 * f.mp * f.np + 4 * f.mp * f.mp);
+    f.vec = c % 4 == 0 && ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(mom)) & 15) == 0;
+    const unsigned lds = (unsigned)ns_fused_bytes(f.mp, f.np);
     hipLaunchKernelGGL(ns_fused_kernel, dim3((unsigned)n), dim3(1024), lds, s, f);
     NSH_LAUNCHED();
     return 0;
