@@ -256,7 +256,8 @@ int nsh_op_adamw_step(float* w, const float* g, float* m, float* v, int64_t n, i
  * 16-byte aligned, of the size that their functions give (0: nothing needed,
  * or sizes that the call refuses); the other buffers at any float.
  *
- * Sizes: E <= 1024 experts, K <= 64 choices, T K <= 2^24 slots. */
+ * Sizes: E <= 1024 experts, K <= 64 choices, T K <= 2^24 slots, and (T K / 128 +
+ * E) blocks of max(D, H) / 128 below 2^21 (2^35 floats of slots). */
 
 /* Routing of T tokens to K of E experts each, from logits [T, E].
  *   score 0: s = softmax of the row over its live experts, 1: s = 1 / (1 + e^-l)

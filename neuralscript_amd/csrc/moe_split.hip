@@ -306,12 +306,13 @@ __global__ __launch_bounds__(256) void turn_kernel(const float* __restrict__ src
                                                    const int* __restrict__ blk, const int* __restrict__ nrows,
                                                    const int* __restrict__ top, _Float16* __restrict__ out, int64_t C,
                                                    int64_t np) {
-  const int64_t p0 = (int64_t)blockIdx.x * kPad;
+  const int ctiles = (int)((C + 63) / 64), b = blockIdx.x / ctiles;
+  const int64_t p0 = (int64_t)b * kPad;
   if (p0 >= *nrows) return;
   const int c = threadIdx.x & 63, o = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.y * 64 + c;
+  const int64_t col = (int64_t)(blockIdx.x % ctiles) * 64 + c;
   if (col >= C) return;
-  const int ex = seg_exp(top[blk[blockIdx.x]]);
+  const int ex = seg_exp(top[blk[b]]);
   float v[8];
 #pragma unroll
   for (int u = 0; u < 8; u++) {
@@ -936,7 +937,7 @@ int launch_experts_split_grad(const float* dy, const float* x, const float* weig
   const int64_t items = moe_bwd_most_items(z.np, m.D, m.H, m.E);
   auto weight_grad = [&](const float* src, const int* top, _Float16* turned, const _Float16* A, const _Float16* B,
                          int64_t M, int64_t N, int back, float* out) -> int {
-    hipLaunchKernelGGL(turn_kernel, dim3((unsigned)(z.np / kPad), (unsigned)ceil_div(m.D, 64)), dim3(256), 0, s, src,
+    hipLaunchKernelGGL(turn_kernel, dim3((unsigned)(z.np / kPad * ceil_div(m.D, 64))), dim3(256), 0, s, src,
                        st.t.tok, st.t.blk, nrows, top, turned, m.D, z.np);
     NSH_LAUNCHED();
     SplitArgs k = with_stats(split_args(m, st, M, act));

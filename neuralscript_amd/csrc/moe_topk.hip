@@ -675,6 +675,7 @@ struct FewArgs {
   const float* W;      // [E, k, cols]
   const int32_t* idx;
   float* out;          // [chunks][slots, cols]
+  float* keep;         // second product: u [slots, k] for the gradient, or null
   int slots, choices, E, k, cols, chunk, parts, act;
   bool by_slot;
 };
@@ -743,6 +744,7 @@ __global__ __launch_bounds__(256) void few_kernel(FewArgs a) {
           } else {
             const float* p = a.in + (int64_t)slot * a.k + k0 + k;
             v = sum_parts(p, (int64_t)a.slots * a.k, a.parts);
+            if (a.keep && blockIdx.x == 0 && r < nr) a.keep[(int64_t)slot * a.k + k0 + k] = v;
             v = act_apply(v, a.act);
           }
           xs[k * R + r] = r < nr ? v : 0.f;
@@ -814,21 +816,206 @@ __global__ __launch_bounds__(256) void few_kernel(FewArgs a) {
   }
 }
 
-// y[t] = sum over the token's slots of weight * (sum over the chunks of o)
+// y[t] = sum over the token's slots of weight * (sum over the chunks of o);
+// expert (not null): the slots' experts for the gradient, -1 where idx is out of
+// range.
 __global__ __launch_bounds__(256) void few_combine_kernel(const float* __restrict__ o, const int32_t* __restrict__ idx,
                                                           const float* __restrict__ weight, float* __restrict__ y,
-                                                          int64_t n, int choices, int cols, int E, int slots,
-                                                          int parts) {
+                                                          int* __restrict__ expert, int64_t n, int choices, int cols,
+                                                          int E, int slots, int parts) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   const int t = (int)(i / cols), c = (int)(i - (int64_t)t * cols);
   float y0 = 0.f;
   for (int k = 0; k < choices; k++) {
     const int slot = t * choices + k, e = idx[slot];
-    if (e < 0 || e >= E) continue;
+    const bool out = e < 0 || e >= E;
+    if (expert && c == 0) expert[slot] = out ? -1 : e;
+    if (out) continue;
     y0 += weight[slot] * sum_parts(o + (int64_t)slot * cols + c, (int64_t)slots * cols, parts);
   }
   y[i] = y0;
+}
+
+// The slots of an expert into `list`, by one wave; their number to *count.
+__device__ __forceinline__ void list_slots(const int* __restrict__ expert, int slots, int e, int* list, int* count) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int s0 = 0; s0 < slots; s0 += 64) {
+    const int s = s0 + lane;
+    const uint64_t m = __ballot(s < slots && expert[min(s, slots - 1)] == e);
+    if ((m >> lane) & 1) list[n + __builtin_popcountll(m & ((1ull << lane) - 1))] = s;
+    n += __builtin_popcountll(m);
+  }
+  if (lane == 0) *count = n;
+}
+
+// out[slot, row] = sum_k in[slot, k] W[e][row, k]: rows of W along the lanes, four
+// rows a wave, up to 8 slots a pass, each row's sums met by wave reductions.
+// in: row slot (choices 0) or slot / choices.
+struct FewRowsArgs {
+  const float* in;
+  const float* W;       // [E, rows, k]
+  const int* expert;    // [slots]
+  float* out;           // [slots, rows]
+  int slots, choices, k, rows, E;
+  bool by_slot;
+};
+template <bool VEC>
+__global__ __launch_bounds__(256) void few_rows_kernel(FewRowsArgs a) {
+  constexpr int R = kFewRows, W4 = VEC ? 4 : 1, CHUNK = 1024, STEPS = CHUNK / (64 * W4);
+  __shared__ int list[kFewSlots];
+  __shared__ int count;
+  __shared__ __attribute__((aligned(16))) float xs[R][CHUNK];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int e = a.by_slot ? a.expert[blockIdx.y] : (int)blockIdx.y;
+  if (e < 0) return;
+  if (w == 0) list_slots(a.expert, a.slots, e, list, &count);
+  __syncthreads();
+  const int n = count;
+  if (n == 0 || (a.by_slot && list[0] != (int)blockIdx.y)) return;
+  const int row0 = blockIdx.x * 16 + w * 4;
+  for (int r0 = 0; r0 < n; r0 += R) {
+    const int nr = min(R, n - r0);
+    float acc[4][R];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int r = 0; r < R; r++) acc[j][r] = 0.f;
+    for (int k0 = 0; k0 < a.k; k0 += CHUNK) {
+      const int kn = min(CHUNK, a.k - k0);
+      __syncthreads();
+      for (int r = 0; r < nr; r++) {
+        const int slot = list[r0 + r], from = a.choices ? slot / a.choices : slot;
+        for (int k = t; k < CHUNK; k += 256) xs[r][k] = k < kn ? a.in[(int64_t)from * a.k + k0 + k] : 0.f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float* __restrict__ p = a.W + ((int64_t)e * a.rows + min(row0 + j, a.rows - 1)) * a.k + k0;
+        float v[STEPS][W4];
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+          const int k = (s * 64 + lane) * W4;
+          const bool in = k < kn;
+          if constexpr (VEC) {
+            const float4 f = *reinterpret_cast<const float4*>(p + (in ? k : 0));
+            v[s][0] = in ? f.x : 0.f; v[s][1] = in ? f.y : 0.f; v[s][2] = in ? f.z : 0.f; v[s][3] = in ? f.w : 0.f;
+          } else {
+            const float f = p[in ? k : 0];
+            v[s][0] = in ? f : 0.f;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          if (r >= nr) break;  // (uniform)
+#pragma unroll
+          for (int s = 0; s < STEPS; s++) {
+            const int k = (s * 64 + lane) * W4;
+            if constexpr (VEC) {
+              const float4 x = *reinterpret_cast<const float4*>(&xs[r][k]);
+              acc[j][r] += (x.x * v[s][0] + x.y * v[s][1]) + (x.z * v[s][2] + x.w * v[s][3]);
+            } else {
+              acc[j][r] += xs[r][k] * v[s][0];
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      if (r >= nr) break;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float d = wave_sum(acc[j][r]);
+        if (lane == j && row0 + j < a.rows) a.out[(int64_t)list[r0 + r] * a.rows + row0 + j] = d;
+      }
+    }
+  }
+}
+
+// One wave a slot: dweight = act(u) . dh, du = weight act'(u) dh (in place of dh),
+// hw = weight act(u); slots without an expert get a dweight of 0.
+__global__ __launch_bounds__(256) void few_back_kernel(const float* __restrict__ u, float* __restrict__ dh,
+                                                       float* __restrict__ hw, const float* __restrict__ weight,
+                                                       float* __restrict__ dweight, const int* __restrict__ expert,
+                                                       int slots, int H, int act) {
+  const int lane = threadIdx.x & 63, slot = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (slot >= slots) return;
+  if (expert[slot] < 0) {
+    if (dweight && lane == 0) dweight[slot] = 0.f;
+    return;
+  }
+  const float w = weight[slot];
+  float dot = 0.f;
+  for (int i = lane; i < H; i += 64) {
+    const int64_t at = (int64_t)slot * H + i;
+    const float d = dh[at];
+    float h, slope;
+    act_both(u[at], act, h, slope);
+    dot += h * d;
+    dh[at] = w * d * slope;
+    hw[at] = w * h;
+  }
+  dot = wave_sum(dot);
+  if (dweight && lane == 0) dweight[slot] = dot;
+}
+
+// C[e] [M, N] = the sum over e's slots of A[slot] (column) B[slot] (row); zeros
+// without slots.  A, B: row slot, or slot / choices where ca, cb.  A workgroup: 16
+// rows by up to 1024 columns (256 without float4), eight rows a thread at a time.
+struct FewOuterArgs {
+  const float* A;
+  const float* B;
+  const int* expert;
+  float* C;
+  int slots, ca, cb, M, N, ctiles;
+};
+template <bool VEC>
+__global__ __launch_bounds__(256) void few_outer_kernel(FewOuterArgs a) {
+  constexpr int W4 = VEC ? 4 : 1, RT = 8;
+  __shared__ int list[kFewSlots];
+  __shared__ int count;
+  const int t = threadIdx.x, e = blockIdx.y;
+  if (t < 64) list_slots(a.expert, a.slots, e, list, &count);
+  __syncthreads();
+  const int n = count, col = (int)(blockIdx.x % a.ctiles * 256 + t) * W4;
+  if (col >= a.N) return;
+  for (int h = 0; h < 2; h++) {
+    const int row0 = (int)(blockIdx.x / a.ctiles) * 16 + h * RT;
+    if (row0 >= a.M) return;
+    float acc[RT][W4];
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+      for (int j = 0; j < W4; j++) acc[r][j] = 0.f;
+    for (int s = 0; s < n; s++) {
+      const int slot = __builtin_amdgcn_readfirstlane(list[s]);
+      const float* __restrict__ p = a.A + (int64_t)(a.ca ? slot / a.ca : slot) * a.M;
+      const float* __restrict__ q = a.B + (int64_t)(a.cb ? slot / a.cb : slot) * a.N + col;
+      float b[W4];
+      if constexpr (VEC) {
+        const float4 f = *reinterpret_cast<const float4*>(q);
+        b[0] = f.x; b[1] = f.y; b[2] = f.z; b[3] = f.w;
+      } else {
+        b[0] = *q;
+      }
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        const float x = p[min(row0 + r, a.M - 1)];  // (uniform)
+#pragma unroll
+        for (int j = 0; j < W4; j++) acc[r][j] = fmaf(x, b[j], acc[r][j]);
+      }
+    }
+    float* __restrict__ c = a.C + (int64_t)e * a.M * a.N + col;
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+      if (row0 + r >= a.M) break;
+      float* to = c + (int64_t)(row0 + r) * a.N;
+      if constexpr (VEC) *reinterpret_cast<float4*>(to) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+      else *to = acc[r][0];
+    }
+  }
 }
 
 constexpr int64_t round64(int64_t n) { return (n + 63) / 64 * 64; }
@@ -950,8 +1137,9 @@ static int few_chunks(int64_t k, int64_t cols, int64_t slots, int64_t E) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, ceil_div(256, wgs)), k / 64));
 }
 
+// state: the slots' experts, then u [N, H] by slot
 static int launch_few(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2,
-                      float* y, const MoeShape& m, int act, void* workspace, hipStream_t s) {
+                      float* y, const MoeShape& m, int act, void* state, void* workspace, hipStream_t s) {
   const int64_t N = m.T * m.K;
   FewArgs a;
   a.slots = (int)N; a.choices = (int)m.K; a.E = (int)m.E; a.idx = idx; a.act = act;
@@ -970,21 +1158,70 @@ static int launch_few(const float* x, const int32_t* idx, const float* weight, c
   };
   float* u = static_cast<float*>(workspace);
   float* o = u + round64(few_chunks(m.D, m.H, N, m.E) * N * m.H);
-  a.in = x; a.out = u; a.parts = 1;
+  a.in = x; a.out = u; a.keep = nullptr; a.parts = 1;
   a.parts = product(std::true_type{}, m.D, m.H, W1);
   NSH_LAUNCHED();
+  int* expert = static_cast<int*>(state);
   a.in = u; a.out = o;
+  a.keep = state ? reinterpret_cast<float*>(expert + round64(N)) : nullptr;
   const int parts = product(std::false_type{}, m.H, m.D, W2);
   NSH_LAUNCHED();
   hipLaunchKernelGGL(few_combine_kernel, dim3((unsigned)ceil_div(m.T * m.D, 256)), dim3(256), 0, s, o, idx, weight, y,
-                     m.T * m.D, (int)m.K, (int)m.D, (int)m.E, (int)N, parts);
+                     expert, m.T * m.D, (int)m.K, (int)m.D, (int)m.E, (int)N, parts);
   NSH_LAUNCHED();
+  return 0;
+}
+
+static int launch_few_grad(const float* dy, const float* x, const float* weight, const float* W1, const float* W2,
+                           const void* state, float* dx, float* dweight, float* dW1, float* dW2, const MoeShape& m,
+                           int act, void* workspace, hipStream_t s) {
+  const int64_t N = m.T * m.K;
+  const int* expert = static_cast<const int*>(state);
+  const float* u = reinterpret_cast<const float*>(expert + round64(N));
+  float* dh = static_cast<float*>(workspace);
+  float* hw = dh + round64(N * m.H);
+  float* slots = hw + round64(N * m.H);
+  auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  auto rows = [&](const float* in, int choices, const float* W, float* out, int64_t k, int64_t nrows) -> int {
+    FewRowsArgs a;
+    a.in = in; a.W = W; a.expert = expert; a.out = out;
+    a.slots = (int)N; a.choices = choices; a.k = (int)k; a.rows = (int)nrows; a.E = (int)m.E;
+    a.by_slot = N < m.E;
+    const dim3 g((unsigned)ceil_div(nrows, 16), (unsigned)std::min(N, m.E));
+    if (k % 4 == 0 && aligned(W)) hipLaunchKernelGGL(few_rows_kernel<true>, g, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(few_rows_kernel<false>, g, dim3(256), 0, s, a);
+    NSH_LAUNCHED();
+    return 0;
+  };
+  auto outer = [&](const float* A, int ca, const float* B, int cb, float* C, int64_t M, int64_t Nc) -> int {
+    FewOuterArgs a;
+    a.A = A; a.B = B; a.expert = expert; a.C = C;
+    a.slots = (int)N; a.ca = ca; a.cb = cb; a.M = (int)M; a.N = (int)Nc;
+    const bool vec = Nc % 4 == 0 && aligned(B) && aligned(C);
+    a.ctiles = (int)ceil_div(Nc, vec ? 1024 : 256);
+    const dim3 g((unsigned)(a.ctiles * ceil_div(M, 16)), (unsigned)m.E);
+    if (vec) hipLaunchKernelGGL(few_outer_kernel<true>, g, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(few_outer_kernel<false>, g, dim3(256), 0, s, a);
+    NSH_LAUNCHED();
+    return 0;
+  };
+  if (rows(dy, (int)m.K, W2, dh, m.D, m.H) != 0) return -1;
+  hipLaunchKernelGGL(few_back_kernel, dim3((unsigned)ceil_div(N, 4)), dim3(256), 0, s, u, dh, hw, weight, dweight,
+                     expert, (int)N, (int)m.H, act);
+  NSH_LAUNCHED();
+  if (dx) {
+    if (rows(dh, 0, W1, slots, m.H, m.D) != 0) return -1;
+    if (launch_combine(slots, expert, dx, m, s) != 0) return -1;
+  }
+  if (dW1 && outer(x, (int)m.K, dh, 0, dW1, m.D, m.H) != 0) return -1;
+  if (dW2 && outer(hw, 0, dy, (int)m.K, dW2, m.H, m.D) != 0) return -1;
   return 0;
 }
 
 // state: the sorted slots' tables, then the pre-activations [T K, H]
 size_t experts_state_bytes(const MoeShape& m) {
   if (split_takes(m)) return split_state_bytes(m);
+  if (few_slots(m)) return 4 * (size_t)(round64(m.T * m.K) + m.T * m.K * m.H);
   const int64_t N = m.T * m.K;
   return 4 * (size_t)(tables_ints(N, m.E) + N * m.H);
 }
@@ -994,13 +1231,14 @@ size_t experts_state_bytes(const MoeShape& m) {
 size_t experts_workspace_bytes(const MoeShape& m, bool grad) {
   if (split_takes(m)) return split_workspace_bytes(m, grad);
   const int64_t N = m.T * m.K;
+  if (few_slots(m)) {
+    const int64_t fwd = round64(few_chunks(m.D, m.H, N, m.E) * N * m.H) + few_chunks(m.H, m.D, N, m.E) * N * m.D;
+    return 4 * (size_t)std::max(fwd, grad ? 2 * round64(N * m.H) + N * m.D : 0);
+  }
   const int64_t fwd = sort_count_ints(N, m.E) + tables_ints(N, m.E) + round64(N * m.H) + N * m.D;
   const int64_t bwd = 2 * round64(N * m.H) + 3 * round64(N * m.D) + round64(moe_bwd_kpart_floats(N, m.D, m.H)) +
                       moe_bwd_kitem_ints(N, m.D, m.H, m.E);
-  const int64_t few = few_slots(m) ? round64(few_chunks(m.D, m.H, N, m.E) * N * m.H) +
-                                         few_chunks(m.H, m.D, N, m.E) * N * m.D
-                                   : 0;
-  return 4 * (size_t)std::max(std::max(fwd, few), grad ? bwd : 0);
+  return 4 * (size_t)std::max(fwd, grad ? bwd : 0);
 }
 
 int launch_experts(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2, float* y,
@@ -1008,7 +1246,7 @@ int launch_experts(const float* x, const int32_t* idx, const float* weight, cons
   const int64_t N = m.T * m.K;
   if (m.T <= 0 || m.D <= 0) return 0;
   if (split_takes(m)) return launch_experts_split(x, idx, weight, W1, W2, y, m, act, state, workspace, s);
-  if (!state && few_slots(m)) return launch_few(x, idx, weight, W1, W2, y, m, act, workspace, s);
+  if (few_slots(m)) return launch_few(x, idx, weight, W1, W2, y, m, act, state, workspace, s);
   int* wi = static_cast<int*>(workspace);
   int* count = wi;
   wi += sort_count_ints(N, m.E);
@@ -1044,6 +1282,7 @@ int launch_experts_grad(const float* dy, const float* x, const float* weight, co
   }
   if (split_takes(m))
     return launch_experts_split_grad(dy, x, weight, W1, W2, state, dx, dweight, dW1, dW2, m, act, workspace, s);
+  if (few_slots(m)) return launch_few_grad(dy, x, weight, W1, W2, state, dx, dweight, dW1, dW2, m, act, workspace, s);
   int* ti = const_cast<int*>(static_cast<const int*>(state));
   const SlotTables t = tables_at(ti, N, m.E);
   const float* pre = reinterpret_cast<const float*>(ti + tables_ints(N, m.E));

@@ -2168,7 +2168,7 @@ static bool moe_shape_ok(int64_t T, int64_t K, int64_t D, int64_t H, int64_t E) 
   if (T < 0 || T > kMoeMaxSlots || K < 1 || K > kMoeMaxChoices || T * K > kMoeMaxSlots || D < 1 || H < 1 || E < 1 ||
       E > kMoeMaxExperts || D > INT32_MAX / 64 || H > INT32_MAX / 64)
     return false;
-  return (ceil_div(T * K, 128) + E) * ceil_div(std::max(D, H), 128) < (1 << 23);
+  return (ceil_div(T * K, 128) + E) * ceil_div(std::max(D, H), 128) < (1 << 21);
 }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
