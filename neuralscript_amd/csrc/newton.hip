@@ -21,8 +21,9 @@
 // 2 k at step k and not below 0 (a step grows X by at most 3.4445), so that its
 // entries keep their bits.
 //
-// Operands are padded with zeros to a contraction length of 32 k.  X is kept both ways, as the Gram product's operand (rows m, contraction N) and as
-// the update's (rows N, contraction m); S and P are symmetric and need one.
+// Operands are padded with zeros to a contraction length of 32 k.  X is kept both
+// ways, as the Gram product's operand (rows m, contraction N) and as the update's
+// (rows N, contraction m); S and P are symmetric and need one.
 #include <algorithm>
 
 #include "common.h"
@@ -93,15 +94,20 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& g, const floatx16 (&ac
     for (int r = 0; r < TM; r++)
 #pragma unroll
       for (int c = 0; c < TN; c++) {
-        const int64_t col = nw + c * 32 + l32;
+        const int64_t col = nw + c * 32 + l32, row0 = mw + r * 32 + 4 * kh;
         if (col >= g.rb) continue;
+        float* p = f + row0 * g.rb + col;
+        float w[16];  // (all loads before the stores, which may alias them for all the compiler knows)
 #pragma unroll
         for (int v = 0; v < 16; v++) {
-          const int64_t row = mw + r * 32 + 8 * (v >> 2) + 4 * kh + (v & 3);
-          if (row >= g.ra) continue;
+          const int dr = 8 * (v >> 2) + (v & 3);
+          w[v] = g.weights && row0 + dr < g.ra ? p[dr * g.rb] : 0.f;
+        }
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+          const int dr = 8 * (v >> 2) + (v & 3);
           const float x = acc[r][c][v] * down;
-          float* p = f + row * g.rb + col;
-          *p = g.weights ? *p - g.le * x - g.decay * *p : x;
+          if (row0 + dr < g.ra) p[dr * g.rb] = g.weights ? w[v] - g.le * x - g.decay * w[v] : x;
         }
       }
     return;
