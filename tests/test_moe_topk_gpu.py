@@ -443,3 +443,26 @@ def test_experts_of_very_small_and_large_values(scale):
     want, off = so.experts(a["x"], a["idx"], a["weight"], a["W1"], a["W2"], 0)
     got = run_experts(a, 4, 0, False)["y"].astype(np.float64)
     assert np.all(np.abs(got - want["y"]) <= off["y"])
+
+
+@pytest.mark.parametrize("T,D,H", [(3, 64, 96), (3, 33, 17), (400, 132, 260), (401, 131, 129)])
+def test_experts_single_gradients_without_a_sort_and_in_pieces(T, D, H, pieces):
+    """The other two ways through a layer; the knob sends the many slots to the pieces."""
+    a = layer(T, 2, D, H, 6, 2, 0.1)
+    every = run_experts(a, 6, 6, True)
+    again = run_experts(a, 6, 6, True)
+    assert all(np.array_equal(every[k], again[k]) for k in every)
+    for only in (("dx",), ("dweight",), ("dW1",), ("dW2",), ("dx", "dW2"), ("dweight", "dW1"), ()):
+        for k, v in run_experts(a, 6, 6, True, grads=only).items():
+            assert np.array_equal(v, every[k]), (only, k)
+
+
+@pytest.mark.parametrize("T", [3, 150, 700])
+def test_experts_a_token_may_ask_one_expert_twice(T, pieces):
+    a = layer(T, 4, 132, 140, 5, 9)
+    a["idx"][:, 1] = a["idx"][:, 0]
+    a["idx"][::3] = a["idx"][::3, :1]
+    want, off = so.experts(a["x"], a["idx"], a["weight"], a["W1"], a["W2"], 5, a["dy"])
+    got = run_experts(a, 5, 5, True)
+    for k in want:
+        within(got[k], want[k], off[k], k)
