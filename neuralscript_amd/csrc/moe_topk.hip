@@ -6,10 +6,18 @@
 //             weight_k = scale s_k (/ sum_j s_j)
 //   layer     y_t = sum_k weight_tk act(x_t W1[e]) W2[e],  e = idx_tk
 //
-// A (token, choice) pair t K + k is a slot.  The layer sorts the slots by
-// expert (stable, so every sum has one order) and runs grouped products over
-// the sorted rows; the slots of a token meet in a pass of their own, in the
-// order of k.
+// A (token, choice) pair t K + k is a slot.  Three ways through the layer, by its
+// sizes alone:
+//  * few slots an expert (few_slots): every workgroup lists its expert's slots and
+//    streams the weights once for up to 8 of them, fp32 multiply-adds; bound by the
+//    weights' bytes.
+//  * many (split_takes, moe_split.hip): products of two fp16 pieces over operands
+//    laid out for them; bound by the matrix cores.
+//  * between: the slots are sorted by expert (stable, so every sum has one order),
+//    and gemm.hip's grouped products (three bf16 pieces) run over the sorted rows,
+//    gathered and scattered as they are; bound by the matrix cores or, in a small
+//    layer, by the latency of some ten launches.
+// The slots of a token meet in a pass of their own, in the order of k.
 #include <algorithm>
 
 #include "common.h"
@@ -208,8 +216,11 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
 //
 // Four tokens a wave: a row of 16 lanes holds a token's experts, V consecutive
 // ones a lane, and reduces over itself by DPP moves alone (a whole wave's
-// butterfly goes through LDS: six round trips a choice).  Bound by the 64-bit
-// arithmetic: 16384 tokens of 256 experts, 8 groups, 8 choices: see launch_route.
+// butterfly goes through LDS: six round trips a choice).  Bound by instruction issue:
+// 16384 tokens, 8 of 256 experts in 8 groups 27 us (57 with a wave a token), 2460
+// vector instructions a wave; the gradient by its bytes, 65536 tokens of 64 experts
+// 9.8 us.  Measured and not kept: the choice in 32 bits first, and in 64 where two
+// values of the order are near each other (30 us).
 template <int CTRL>
 __device__ __forceinline__ int dpp_int(int v) {
   return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, true);
@@ -661,11 +672,11 @@ __global__ __launch_bounds__(256) void gather_kernel(const float* __restrict__ a
 // rows cost a quarter of the time that the weights take to arrive).  Workgroup
 // (column tile, expert, K chunk) lists the expert's slots itself and streams 64
 // columns of its chunk once for up to 8 of them (with fewer slots than experts:
-// (column tile, slot, K chunk), and the first of an expert's slots does it); the chunks make enough
-// workgroups to fill the chip and are summed, in their order, by whoever reads
-// them: the second product as it stages act(u), the last pass as it weighs the
-// slots.  64 experts of 1024 x 1024: one token (2 slots) and 37 tokens, us: the
-// sorted products above 186, 197.
+// (column tile, slot, K chunk), and the first of an expert's slots does it).  The
+// chunks make enough workgroups to fill the chip and are summed, in their order, by
+// whoever reads them: the second product as it stages act(u), the last pass as it
+// weighs the slots.  64 experts of 1024 x 1024, two slots a token: one token 12 us
+// (sorted 186), 37 tokens 90 us, 4.1 TB/s of weights (sorted 197).
 constexpr int kFewSlots = 1024;  // most slots (a list in LDS)
 constexpr int kFewRows = 8;      // rows a pass over the weights
 constexpr int kFewK = 512;       // contraction staged at once

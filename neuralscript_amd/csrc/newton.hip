@@ -528,7 +528,7 @@ __global__ __launch_bounds__(256) void ns_normalise_kernel(const float* g, const
 // spread over the banks): up to 64 x 256.  A step is three products with a barrier
 // between: S and P in 16 x 16 blocks (of 32 x 32 most waves would have none), X in
 // 32 x 32 ones (half of the LDS reads).  Bound by LDS traffic and the waves'
-// latency: 8 of 64 x 256 in 5 steps: see launch_newton_schulz.
+// latency: 8 of 64 x 256 in 5 steps 35 us (84 with a launch for each product).
 constexpr int kNsLds = 163840;
 struct NsFused {
   const float* g;
