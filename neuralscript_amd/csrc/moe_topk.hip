@@ -155,6 +155,35 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
   }
 }
 
+// The gradient that one choice hands its own logit, in every mode but the softmax
+// without renorm (whose sum reaches all experts): u = scale dweight, x the choice's
+// logit (some: live, else u is 0), mx the token's largest.
+//   sigmoid           u s (1 - s)
+//   renorm, softmax   w (u - sum_j w_j u_j), w = s / sum_j s_j = e^(x - top) / sum_j ..
+//   renorm, sigmoid   the same, times 1 - s
+// 1 - s is taken from e^-|x|, and the shares w from differences to the largest
+// chosen logit: neither cancels nor underflows where 1 - s or s do.  A sum of the
+// scores that is 0 in 64 bits made weights of 0, whose gradient is 0.
+template <class Sum, class Max>
+__device__ __forceinline__ float choice_grad(bool some, float x, float u, float mx, int score, int renorm, Sum sum,
+                                             Max max) {
+  x = some ? x : 0.f;
+  const float t = expf(-fabsf(x)), inv = 1.f / (1.f + t);
+  if (!renorm) return u * (t * inv * inv);
+  const float top = max(some ? x : -__builtin_inff());
+  float f;
+  if (score) f = x > 0.f ? inv : expf(x - fminf(top, 0.f)) * inv;  // s e^-min(top, 0)
+  else f = x == top ? 1.f : expf(x - top);
+  f = some ? f : 0.f;
+  const float total = sum(f);
+  const float w = total > 0.f ? f / total : 0.f;
+  const float dot = sum(w * u);
+  float g = w * (u - dot);
+  if (score) g *= x > 0.f ? t * inv : inv;
+  const bool none = score ? top < -709.78f : top - mx < -745.13f;
+  return (int)some & (int)!none ? g : 0.f;
+}
+
 // One wave per token; lane k holds choice k.
 template <int V>
 __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
@@ -162,38 +191,40 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
   const int64_t tok = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (tok >= a.T) return;
   const float* __restrict__ l = a.logits + tok * a.E;
-  float x[V], s[V], mx = -__builtin_inff(), sum = 0.f;
+  float x[V], s[V], mx = -__builtin_inff();
 #pragma unroll
   for (int v = 0; v < V; v++) {
     x[v] = live_logit(l, v * 64 + lane, a.E, a.active);
     mx = fmaxf(mx, x[v]);
   }
   mx = wave_max(mx);
-#pragma unroll
-  for (int v = 0; v < V; v++) {
-    const bool live = x[v] > -__builtin_inff();
-    s[v] = !live ? 0.f : a.score ? 1.f / (1.f + expf(-x[v])) : x[v] == mx ? 1.f : expf(x[v] - mx);
-    sum += s[v];
-  }
-  const float by = a.score ? 1.f : wave_sum(sum);
-  // this lane's choice, its score and the derivative by that score
+  // this lane's choice
   int mine = -1;
-  float u = 0.f, sk = 0.f;
-  float xm = -__builtin_inff();
+  float u = 0.f, xm = -__builtin_inff();
   if (lane < a.K) {
     mine = a.idx[tok * a.K + lane];
     xm = live_logit(l, mine, a.E, a.active);
   }
-  mine = xm > -__builtin_inff() ? mine : -1;
-  if (mine >= 0) {
-    sk = a.score ? 1.f / (1.f + expf(-xm)) : (xm == mx ? 1.f : expf(xm - mx)) / by;
-    u = a.dweight[tok * a.K + lane] * a.scale;
+  const bool some = xm > -__builtin_inff();
+  mine = some ? mine : -1;
+  if (some) u = a.dweight[tok * a.K + lane] * a.scale;
+  const bool spread = !a.score && !a.renorm;  // (uniform) the softmax's sum reaches every expert
+  float dot = 0.f;
+  if (spread) {
+    float sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      s[v] = !(x[v] > -__builtin_inff()) ? 0.f : x[v] == mx ? 1.f : expf(x[v] - mx);
+      sum += s[v];
+    }
+    const float by = wave_sum(sum), p = by > 0.f ? 1.f / by : 0.f;  // (0: no expert is live)
+#pragma unroll
+    for (int v = 0; v < V; v++) s[v] *= p;
+    dot = wave_sum(some ? u * ((xm == mx ? 1.f : expf(xm - mx)) * p) : 0.f);
+  } else {
+    u = choice_grad(some, xm, u, mx, a.score, a.renorm, [](float v) { return wave_sum(v); },
+                    [](float v) { return wave_max(v); });
   }
-  if (a.renorm) {
-    const float total = wave_sum(sk), dot = wave_sum(u * sk);
-    u = mine >= 0 && total > 0.f ? (u - dot / total) / total : 0.f;
-  }
-  const float dot = a.score ? 0.f : wave_sum(u * sk);
   float ds[V];
 #pragma unroll
   for (int v = 0; v < V; v++) ds[v] = 0.f;
@@ -206,9 +237,7 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
 #pragma unroll
   for (int v = 0; v < V; v++) {
     const int e = v * 64 + lane;
-    if (e >= a.E) continue;
-    const float p = by > 0.f ? s[v] / by : 0.f;  // (0: no expert is live)
-    a.dlogits[tok * a.E + e] = a.score ? p * (1.f - p) * ds[v] : p * (ds[v] - dot);
+    if (e < a.E) a.dlogits[tok * a.E + e] = spread ? s[v] * (ds[v] - dot) : ds[v];
   }
 }
 
@@ -422,29 +451,32 @@ __global__ __launch_bounds__(256) void route_grad_row_kernel(RouteGradArgs a) {
     mine = a.idx[tok * a.K + lane];
     dw = a.dweight[tok * a.K + lane];
   }
-  float x[V], s[V], mx = -__builtin_inff(), sum = 0.f;
+  float x[V], s[V], mx = -__builtin_inff();
   live_logits<V, VEC>(l, e0, a.E, a.active, x);
   xm = live_logit(l, mine, a.E, a.active);
 #pragma unroll
   for (int v = 0; v < V; v++) mx = fmaxf(mx, x[v]);
   mx = row_max(mx);
-#pragma unroll
-  for (int v = 0; v < V; v++) {
-    const bool live = x[v] > -__builtin_inff();
-    s[v] = !live ? 0.f : a.score ? 1.f / (1.f + expf(-x[v])) : x[v] == mx ? 1.f : expf(x[v] - mx);
-    sum += s[v];
-  }
-  const float by = a.score ? 1.f : row16_sum(sum);
   const bool some = xm > -__builtin_inff();  // (false without a choice: mine -1 is not live)
   mine = some ? mine : -1;
-  float sk = a.score ? 1.f / (1.f + expf(-xm)) : (xm == mx ? 1.f : expf(xm - mx)) / by;
-  sk = some ? sk : 0.f;
   float u = some ? dw * a.scale : 0.f;
-  if (a.renorm) {
-    const float total = row16_sum(sk), dot = row16_sum(u * sk);
-    u = (int)some & (int)(total > 0.f) ? (u - dot / total) / total : 0.f;
+  const bool spread = !a.score && !a.renorm;
+  float dot = 0.f;
+  if (spread) {
+    float sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      s[v] = !(x[v] > -__builtin_inff()) ? 0.f : x[v] == mx ? 1.f : expf(x[v] - mx);
+      sum += s[v];
+    }
+    const float by = row16_sum(sum), p = by > 0.f ? 1.f / by : 0.f;
+#pragma unroll
+    for (int v = 0; v < V; v++) s[v] *= p;
+    dot = row16_sum(some ? u * ((xm == mx ? 1.f : expf(xm - mx)) * p) : 0.f);
+  } else {
+    u = choice_grad(some, xm, u, mx, a.score, a.renorm, [](float v) { return row16_sum(v); },
+                    [](float v) { return row_max(v); });
   }
-  const float dot = a.score ? 0.f : row16_sum(u * sk);
   float ds[V];
 #pragma unroll
   for (int v = 0; v < V; v++) ds[v] = 0.f;
@@ -455,12 +487,8 @@ __global__ __launch_bounds__(256) void route_grad_row_kernel(RouteGradArgs a) {
 #pragma unroll
     for (int v = 0; v < V; v++) ds[v] += e == v ? d : 0.f;
   }
-  const float p1 = by > 0.f ? 1.f / by : 0.f;  // (0: no expert is live)
 #pragma unroll
-  for (int v = 0; v < V; v++) {
-    const float p = s[v] * p1;
-    ds[v] = a.score ? p * (1.f - p) * ds[v] : p * (ds[v] - dot);
-  }
+  for (int v = 0; v < V; v++) ds[v] = spread ? s[v] * (ds[v] - dot) : ds[v];
   if (!in) return;
   float* __restrict__ to = a.dlogits + tok * a.E;
   if constexpr (VEC) {

@@ -174,6 +174,48 @@ def test_route_grad_of_any_choice(score, renorm):
     assert np.all(got[3] == 0)
 
 
+@pytest.mark.parametrize("E,K", [(24, 6), (200, 3), (300, 6), (1024, 20)])
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("renorm", [0, 1])
+@pytest.mark.parametrize("at", [-600.0, -300.0, -110.0, -60.0, 12.0, 40.0])
+def test_route_grad_far_from_zero(E, K, score, renorm, at):
+    """Chosen scores that underflow in 32 bits (a bias or a group can choose
+    experts far below the best) and sigmoids next to 1, element by element."""
+    rng = np.random.default_rng(int(abs(at)) + E)
+    T = 7
+    l = (at + rng.normal(size=(T, E))).astype(np.float32)
+    if score == 0 and at < 0:
+        l[:, 0] = 1.0  # the best expert, which no token chose
+    idx = np.stack([rng.permutation(np.arange(1, E))[:K] for _ in range(T)]).astype(np.int32)
+    dw = rng.normal(size=(T, K)).astype(np.float32)
+    out = Guarded(T * E)
+    d = [put(dw), put(l), put(idx, np.int32)]
+    runtime.op("moe_route_grad", p(d[0]), p(d[1]), None, p(d[2]), p(out), T, E, K, score, renorm, 1.5, None)
+    so.sync()
+    got = out.host((T, E)).astype(np.float64)
+    x, u = np.take_along_axis(l, idx, 1).astype(np.float64), 1.5 * dw.astype(np.float64)
+    left = 1 / (1 + np.exp(x)) if score else 1.0  # 1 - s
+    want, size = np.zeros((T, E)), np.zeros((T, E))
+    if renorm:
+        s = np.exp(x - x.max(1, keepdims=True)) * left if score else np.exp(x - x.max(1, keepdims=True))
+        w = s / s.sum(1, keepdims=True)
+        g = w * (u - (w * u).sum(1, keepdims=True)) * left
+        big = w * (np.abs(u) + (w * np.abs(u)).sum(1, keepdims=True)) * left
+    elif score:
+        g = np.exp(x) * left * left * u
+        big = np.abs(g)
+    else:
+        want, size = so.route_grad(dw, l, None, idx, 0, 0, 1.5)
+    if renorm or score:
+        np.put_along_axis(want, idx, g, 1)
+        np.put_along_axis(size, idx, big, 1)
+    # a rounded difference of logits that are within 8 of each other (a whole logit
+    # without renorm) in each exponential, twice, and the sums over K
+    z = 8 if renorm else np.abs(l).max()
+    off = (8 * (z + 2) + K + 100) * U * size + 1e-37
+    assert np.all(np.abs(got - want) <= off), (np.abs(got - want) / off).max()
+
+
 # ---- the experts' products ----------------------------------------------------------
 
 def layer(T, K, D, H, E, seed, empty=0.0, skew=0.0):
