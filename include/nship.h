@@ -292,9 +292,11 @@ int nsh_op_moe_route_grad(const float* dweight, const float* logits, const uint8
  * same expert may stand in several slots of a token.  The sums' order depends
  * on the sizes and idx alone: equal calls give equal bits.
  * Accuracy: fp32 sums.  A layer with hundreds of slots an expert takes the
- * products' operands as 22 bits of each entry, down to 2^-17 of the largest of
- * its row (of x, act(u), dy and du a slot, of the weights a column of an
- * expert's matrix), and below that as an absolute 2^-40 of it; others as 24.
+ * products' operands as 22 bits of each entry, down to 2^-17 of a scale, and
+ * below that as an absolute 2^-40 of it: the largest entry of the slot's row of x
+ * or dy and of the expert matrix's row or column that is summed over; for act(u)
+ * and du the product of the two operands' 2-norms; in the weights' gradients the
+ * largest of these over the expert's slots.  Other layers take 24 bits.
  * state (NULL for inference): keeps what the gradient needs. */
 size_t nsh_op_moe_experts_state(int64_t T, int64_t K, int64_t D, int64_t H, int64_t E);
 size_t nsh_op_moe_experts_workspace(int64_t T, int64_t K, int64_t D, int64_t H, int64_t E, int grad);

@@ -829,7 +829,8 @@ int launch_product(NsArgs& g, hipStream_t s) {
   const double k = (double)g.k;
   const double t32 = (double)tiles(32, 32), t64 = (double)tiles(64, 64);
   const int64_t n128 = ceil_div(tiles(128, 128), 256), n256 = ceil_div(tiles(256, 256), 256);
-  const double us[4] = {std::max(4 + 0.0031 * k, 3 + 2.2e-5 * k * t32), std::max(6 + 0.0075 * k, 3 + 6.5e-5 * k * t64),
+  // (32 x 32 at most 2^22 workgroups: a launch takes fewer than 2^32 threads)
+  const double us[4] = {t32 > 0x1p22 ? 1e30 : std::max(4 + 0.0031 * k, 3 + 2.2e-5 * k * t32), std::max(6 + 0.0075 * k, 3 + 6.5e-5 * k * t64),
                         9 + 0.0215 * k * (n128 == 1 ? 1. : 1.2 * n128), 8 + 0.095 * k * n256};
   const int64_t side[4] = {32, 64, 128, 256};
   const int use = (int)(std::min_element(us, us + 4) - us);
