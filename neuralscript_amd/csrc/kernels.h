@@ -338,6 +338,17 @@ int launch_experts_split_grad(const float* dy, const float* x, const float* weig
                               const void* state, float* dx, float* dweight, float* dW1, float* dW2, const MoeShape& m,
                               int act, void* workspace, hipStream_t s);
 
+// moe_small.hip: both products of the sorted slots at once, for layers and
+// pointers that small_takes; slots [T K, D] as launch_combine takes them.  pre
+// [T K, H] by position (forward: may be null); xs, dys null: the rows for the
+// weights' gradients are not wanted (dh, hw, xs, dys).
+bool small_takes(const MoeShape& m, const void* x, const void* W1, const void* W2);
+int launch_small(const float* x, const float* weight, const float* W1, const float* W2, const SlotTables& t, float* pre,
+                 float* slots, const MoeShape& m, int act, hipStream_t s);
+int launch_small_grad(const float* dy, const float* x, const float* weight, const float* W1, const float* W2,
+                      const SlotTables& t, const float* pre, float* dh, float* hw, float* xs, float* dys, float* dweight,
+                      float* slots, const MoeShape& m, int act, hipStream_t s);
+
 // newton.hip -------------------------------------------------------------------
 // Orthogonalisation of n matrices [r, c] by `steps` Newton-Schulz products.
 // step null: q = the result of g.  Else the Muon update: m = mu m + g (m not

@@ -13,10 +13,11 @@
 //    weights' bytes.
 //  * many (split_takes, moe_split.hip): products of two fp16 pieces over operands
 //    laid out for them; bound by the matrix cores.
-//  * between: the slots are sorted by expert (stable, so every sum has one order),
-//    and gemm.hip's grouped products (three bf16 pieces) run over the sorted rows,
-//    gathered and scattered as they are; bound by the matrix cores or, in a small
-//    layer, by the latency of some ten launches.
+//  * between: the slots are sorted by expert (stable, so every sum has one order).
+//    A small layer's two products run in one kernel (small_takes, moe_small.hip),
+//    bound by the latency of some ten launches; else gemm.hip's grouped products
+//    (three bf16 pieces) run over the sorted rows, gathered and scattered as they
+//    are, bound by the matrix cores.
 // The slots of a token meet in a pass of their own, in the order of k.
 #include <algorithm>
 
@@ -1295,6 +1296,11 @@ int launch_experts(const float* x, const int32_t* idx, const float* weight, cons
   float* slots = hidden + round64(N * m.H);
   const SlotTables t = tables_at(ti, N, m.E);
   if (launch_sort_slots(idx, t, count, N, (int)m.K, (int)m.E, 1, 128, 0, s) != 0) return -1;
+  if (small_takes(m, x, W1, W2)) {
+    float* pre = state ? reinterpret_cast<float*>(ti + tables_ints(N, m.E)) : nullptr;
+    if (launch_small(x, weight, W1, W2, t, pre, slots, m, act, s) != 0) return -1;
+    return launch_combine(slots, t.expert, y, m, s);
+  }
   GemmArgs g = grouped(t, N, m.H, m.D, x, W1, hidden, m, false);
   g.a_rows = t.tok;
   g.act = act;
@@ -1333,10 +1339,25 @@ int launch_experts_grad(const float* dy, const float* x, const float* weight, co
   float* kpart = slots + round64(N * m.D);
   int* kitems = reinterpret_cast<int*>(kpart + round64(moe_bwd_kpart_floats(N, m.D, m.H)));
   const int* nrows = t.seg + m.E;
+  if (dweight && launch_fill(dweight, N, 0.f, s) != 0) return -1;
+  // the two products of the weights' gradients, from rows by position
+  auto weight_grads = [&]() -> int {
+    if (!dW1 && !dW2) return 0;
+    if (launch_moe_kitems(t.seg, kitems, nullptr, N, m.D, m.H, m.E, s) != 0) return -1;
+    if (dW1 && launch_moe_weight_grad(xs, dh, dW1, m.D, m.H, kitems, kpart, N, m.D, m.H, m.E, s) != 0) return -1;
+    return dW2 ? launch_moe_weight_grad(hw, dys, dW2, m.H, m.D, kitems, kpart, N, m.D, m.H, m.E, s) : 0;
+  };
+  if (small_takes(m, dy, W1, W2) && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+    const bool rows = dW1 || dW2;
+    if (launch_small_grad(dy, x, weight, W1, W2, t, pre, dh, hw, rows ? xs : nullptr, rows ? dys : nullptr, dweight,
+                          dx ? slots : nullptr, m, act, s) != 0)
+      return -1;
+    if (dx && launch_combine(slots, t.expert, dx, m, s) != 0) return -1;
+    return weight_grads();
+  }
   GemmArgs g = grouped(t, N, m.H, m.D, dy, W2, dh, m, true);
   g.a_rows = t.tok;
   if (launch_gemm_ex(g, false, true, 1, s) != 0) return -1;
-  if (dweight && launch_fill(dweight, N, 0.f, s) != 0) return -1;
   hipLaunchKernelGGL(bwd_rows_kernel, dim3((unsigned)ceil_div(N, 4)), dim3(256), 0, s, pre, dh, hw, weight, dweight,
                      t.perm, nrows, (int)m.H, act);
   NSH_LAUNCHED();
@@ -1349,10 +1370,7 @@ int launch_experts_grad(const float* dy, const float* x, const float* weight, co
   if (!dW1 && !dW2) return 0;
   hipLaunchKernelGGL(gather_kernel, dim3(stream_blocks(N * m.D)), dim3(256), 0, s, x, dy, t.tok, nrows, xs, dys, m.D);
   NSH_LAUNCHED();
-  if (launch_moe_kitems(t.seg, kitems, nullptr, N, m.D, m.H, m.E, s) != 0) return -1;
-  if (dW1 && launch_moe_weight_grad(xs, dh, dW1, m.D, m.H, kitems, kpart, N, m.D, m.H, m.E, s) != 0) return -1;
-  if (dW2 && launch_moe_weight_grad(hw, dys, dW2, m.H, m.D, kitems, kpart, N, m.D, m.H, m.E, s) != 0) return -1;
-  return 0;
+  return weight_grads();
 }
 
 }  // namespace nship

@@ -508,3 +508,63 @@ def test_experts_a_token_may_ask_one_expert_twice(T, pieces):
     got = run_experts(a, 5, 5, True)
     for k in want:
         within(got[k], want[k], off[k], k)
+
+
+# both products in one workgroup: sizes around its 32 rows, 8 columns a step, 32
+# columns a block and every division of the second product among eight waves
+SMALL = [(60, 2, 4, 4, 2, 0.0), (33, 1, 8, 12, 1, 0.0), (97, 2, 12, 20, 3, 0.1), (64, 1, 36, 28, 2, 0.0),
+         (150, 3, 64, 36, 5, 0.2), (128, 2, 68, 100, 4, 0.0), (90, 2, 100, 256, 3, 0.0), (129, 1, 132, 128, 1, 0.0),
+         (200, 2, 160, 260, 7, 0.0), (77, 4, 224, 64, 9, 0.3), (161, 1, 256, 512, 4, 0.0), (1024, 2, 256, 132, 3, 0.0)]
+
+
+@pytest.mark.parametrize("T,K,D,H,E,empty", SMALL)
+@pytest.mark.parametrize("act", [1, 5])
+def test_experts_of_a_small_layer(T, K, D, H, E, empty, act):
+    print(f"experts {T} {K} {D} {H} {E} {act}", flush=True)
+    a = layer(T, K, D, H, E, T + D + H, empty, 0.3)
+    want, off = so.experts(a["x"], a["idx"], a["weight"], a["W1"], a["W2"], act, a["dy"])
+    got = run_experts(a, E, act, True)
+    for k in want:
+        within(got[k], want[k], off[k], k)
+    assert np.array_equal(run_experts(a, E, act, False)["y"], got["y"])
+    bad = (a["idx"] < 0) | (a["idx"] >= E)
+    assert np.all(got["dweight"][bad] == 0)
+    for only in (("dx",), ("dweight",), ("dW2",)):
+        assert np.array_equal(run_experts(a, E, act, True, grads=only)[only[0]], got[only[0]])
+
+
+def test_experts_of_a_small_layer_keep_infinities_apart():
+    a = layer(70, 2, 64, 96, 4, 8)
+    a["idx"] %= 3
+    a["W1"][3], a["W2"][3] = np.nan, np.inf
+    a["x"][5, 3] = np.inf
+    a["W2"][a["idx"][5, 0], 2, 3] = np.inf
+    got = run_experts(a, 4, 5, True)
+    plain = dict(a, x=a["x"].copy())
+    plain["x"][5] = 0
+    clean = (a["idx"] != a["idx"][5, 0]).all(1) & (np.arange(70) != 5)
+    want, off = so.experts(plain["x"][clean], a["idx"][clean], a["weight"][clean], a["W1"][:3], a["W2"][:3], 5,
+                           a["dy"][clean])
+    for k in ("y", "dx", "dweight"):
+        within(got[k][clean], want[k], off[k], k)
+    assert not np.isfinite(got["y"][5]).all()
+
+
+# sorted slots of layers that are neither small nor of many slots: wide ones with one
+# side up to 128 (tiles of 128 columns) or above, and a small layer of many slots
+SORTED = [(300, 2, 260, 512, 4, 0.0), (500, 2, 512, 264, 16, 0.1), (300, 2, 640, 128, 8, 0.1), (260, 1, 128, 516, 3, 0.0),
+          (8300, 2, 128, 256, 8, 0.0)]
+
+
+@pytest.mark.parametrize("T,K,D,H,E,empty", SORTED)
+@pytest.mark.parametrize("act", [2, 6])
+def test_experts_of_a_wide_layer(T, K, D, H, E, empty, act):
+    print(f"experts {T} {K} {D} {H} {E} {act}", flush=True)
+    a = layer(T, K, D, H, E, T + D + H, empty, 0.2)
+    want, off = so.experts(a["x"], a["idx"], a["weight"], a["W1"], a["W2"], act, a["dy"])
+    got = run_experts(a, E, act, True)
+    for k in want:
+        within(got[k], want[k], off[k], k)
+    assert np.array_equal(run_experts(a, E, act, False)["y"], got["y"])
+    for only in (("dx",), ("dweight",), ("dW1",)):
+        assert np.array_equal(run_experts(a, E, act, True, grads=only)[only[0]], got[only[0]])

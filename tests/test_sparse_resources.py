@@ -11,7 +11,7 @@ from neuralscript_amd import build
 from test_kernel_resources import _kernel_metadata
 
 SOURCES = {"moe_topk.hip": ("route_row_kernel", "route_grad_row_kernel", "few_kernel", "few_outer_kernel"),
-           "moe_split.hip": ("split_kernel",),
+           "moe_small.hip": ("small_kernel",), "moe_split.hip": ("split_kernel",),
            "newton.hip": ("ns_gemm_kernel", "ns_mid_kernel", "ns_few_kernel", "ns_fused_kernel")}
 
 pytestmark = pytest.mark.skipif(shutil.which("hipcc") is None, reason="hipcc not installed")
