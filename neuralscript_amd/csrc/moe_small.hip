@@ -59,23 +59,30 @@ __device__ __forceinline__ floatx16 block_product(const float* a, const float* _
   for (int v = 0; v < 16; v++) acc[v] = 0.f;
   const int c = min(col, ncols - 1);
   const float* __restrict__ p = TURNED ? W + (int64_t)c * K : W + c;
-#pragma unroll 4
-  for (int k = k0; k < k1; k += 8) {
-    const int at = k + 4 * kh;
-    const bool in = at < K;
-    const int from = in ? at : K - 4;
-    float b[4];
-    if constexpr (TURNED) {
-      const float4 f = *reinterpret_cast<const float4*>(p + from);
-      b[0] = f.x; b[1] = f.y; b[2] = f.z; b[3] = f.w;
-    } else {
+  for (int kk = k0; kk < k1; kk += 64) {
+    float b[8][4];  // (64 steps of K in flight: a round trip to the L2 is longer than their products)
 #pragma unroll
-      for (int j = 0; j < 4; j++) b[j] = p[(int64_t)(from + j) * ncols];
+    for (int o = 0; o < 8; o++) {
+      const int from = min(kk + 8 * o + 4 * kh, K - 4);
+      if constexpr (TURNED) {
+        const float4 f = *reinterpret_cast<const float4*>(p + from);
+        b[o][0] = f.x; b[o][1] = f.y; b[o][2] = f.z; b[o][3] = f.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) b[o][j] = p[(int64_t)(from + j) * ncols];
+      }
     }
-    const float4 x = *reinterpret_cast<const float4*>(a + at);
-    const float xs[4] = {x.x, x.y, x.z, x.w};
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(xs[j], in ? b[j] : 0.f, acc, 0, 0, 0);
+    for (int o = 0; o < 8; o++) {
+      if (kk + 8 * o >= k1) break;  // (uniform)
+      const int at = kk + 8 * o + 4 * kh;
+      const bool in = at < K;
+      const float4 x = *reinterpret_cast<const float4*>(a + at);
+      const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(xs[j], in ? b[o][j] : 0.f, acc, 0, 0, 0);
+    }
   }
   return acc;
 }
