@@ -224,9 +224,9 @@ int launch(SmallArgs g, const SlotTables& t, const MoeShape& m, hipStream_t s) {
 // read the expert's weights from the L2, and the rate of fp32 matrix instructions is
 // below that of three bf16 pieces.  Grouped products -> this, us, forward and
 // training step, (tokens, choices, D, H, experts): 128, 4, 64, 256, 8: 56, 136 ->
-// 27, 81; 1501: 59, 168 -> 31, 107; 32768: 186, 837 -> 170, 829.  1500, 2, 128, 256,
-// 8: 64, 168 -> 34, 113; 16384: 104, 314 -> 94, 326; 65536: 239, 957 -> 278, 1108.
-// 1500, 2, 256, 512, 8: 99, 274 -> 95, 262; 4000: 104, 308 -> 161, 421.
+// 27, 81; 1501: 59, 168 -> 29, 105; 32768: 186, 837 -> 168, 816.  1500, 2, 128, 256,
+// 8: 64, 168 -> 33, 112; 16384: 104, 314 -> 94, 326; 65536: 239, 957 -> 278, 1108.
+// 1500, 2, 256, 512, 8: 99, 274 -> 89, 253; 4000: 104, 308 -> 161, 421.
 bool small_takes(const MoeShape& m, const void* x, const void* W1, const void* W2) {
   if (m.D > 64 && m.T * m.K * m.D * m.H > (1 << 29)) return false;
   return m.D <= kMaxD && m.H <= kMaxH && m.D % 4 == 0 && m.H % 4 == 0 && aligned(x) && aligned(W1) && aligned(W2);
