@@ -281,15 +281,10 @@ def _plain(st):
 
 # ---- the framework's entry points ---------------------------------------------------
 
-_room = {}
-
-
 def _workspace(nbytes):
-    """One workspace for every call, grown where a call needs more."""
-    if _room.get("bytes", -1) < nbytes:
-        _room["buffer"] = torch.empty(max(1, nbytes), device=DEV, dtype=torch.uint8)
-        _room["bytes"] = nbytes
-    return _room["buffer"].data_ptr()
+    """A workspace of the call's own, on the current device and ordered on the current stream as the
+    outputs are: calls on two streams or devices, or captured into two graphs, share none."""
+    return torch.empty(nbytes, device=DEV, dtype=torch.uint8)
 
 
 def _own(st):
@@ -325,21 +320,21 @@ def _own(st):
         if train:
             state = torch.empty(lib.nsh_op_moe_experts_state(*sizes), device=DEV, dtype=torch.uint8)
         rt.op("moe_experts", ptr(st["x"]), ptr(st["idx"]), ptr(st["weight"]), ptr(st["w1"]), ptr(st["w2"]), ptr(y),
-              *sizes, case["act"], ptr(state), ws, stream)
+              *sizes, case["act"], ptr(state), ptr(ws), stream)
         if not train:
             return y
         dx, dweight = torch.empty_like(st["x"]), torch.empty_like(st["weight"])
         dw1, dw2 = torch.empty_like(st["w1"]), torch.empty_like(st["w2"])
         rt.op("moe_experts_grad", ptr(st["dy"]), ptr(st["x"]), ptr(st["weight"]), ptr(st["w1"]), ptr(st["w2"]),
-              ptr(state), ptr(dx), ptr(dweight), ptr(dw1), ptr(dw2), *sizes, case["act"], ws, stream)
+              ptr(state), ptr(dx), ptr(dweight), ptr(dw1), ptr(dw2), *sizes, case["act"], ptr(ws), stream)
         return y, dx, dweight, dw1, dw2
     n, r, c = case["n"], case["r"], case["c"]
     ws = _workspace(lib.nsh_op_newton_schulz_workspace(n, r, c))
     if kind == "ns":
         q = torch.empty_like(st["g"])
-        rt.op("newton_schulz", ptr(st["g"]), ptr(q), n, r, c, STEPS, ws, stream)
+        rt.op("newton_schulz", ptr(st["g"]), ptr(q), n, r, c, STEPS, ptr(ws), stream)
         return q
-    rt.op("muon_ns_step", ptr(st["w"]), ptr(st["g"]), ptr(st["m"]), n, r, c, LR, MU, 1, STEPS, ws, stream)
+    rt.op("muon_ns_step", ptr(st["w"]), ptr(st["g"]), ptr(st["m"]), n, r, c, LR, MU, 1, STEPS, ptr(ws), stream)
     return st["w"], st["m"]
 
 
