@@ -330,6 +330,7 @@ int launch_experts_grad(const float* dy, const float* x, const float* weight, co
 // moe_split.hip: the same for layers that split_takes (by their sizes alone, so
 // that the gradient follows its forward).
 bool split_takes(const MoeShape& m);
+void set_split_least(int64_t slots);  // (tests: see nsh_test_moe_split_least)
 size_t split_state_bytes(const MoeShape& m);
 size_t split_workspace_bytes(const MoeShape& m, bool grad);
 int launch_experts_split(const float* x, const int32_t* idx, const float* weight, const float* W1, const float* W2,

@@ -27,7 +27,7 @@
 // x and dy gathered by position, and for the gradient both once more with
 // positions as k.  They are bound by HBM.
 #include <algorithm>
-#include <cstdlib>
+#include <atomic>
 
 #include "common.h"
 #include "kernels.h"
@@ -732,7 +732,12 @@ int preset(int* p, int64_t n, hipStream_t s) {
 
 bool sigmoid_bound(int act) { return act == kActSigmoid; }
 
+// Tests' choice of the least slots an expert (any size above 128); 0: the rule.
+std::atomic<int64_t> g_split_least{0};
+
 }  // namespace
+
+void set_split_least(int64_t slots) { g_split_least.store(std::max<int64_t>(0, slots), std::memory_order_relaxed); }
 
 // Both products on pieces cost the layouts of the weights (24 bytes an element,
 // forward) and some 50 us of passes, and save half of the products' time.  Sorted
@@ -742,11 +747,10 @@ bool sigmoid_bound(int act) { return act == kActSigmoid; }
 // 298, 839 -> 292, 807.  8 of 256 x 256, 1024: 85, 222 -> 133, 357.  Where a size is
 // no multiple of 4 the others read it float by float: 10 of 200 x 333, 96: 118, 282
 // -> 117, 300; 192: 124, 323 -> 121, 317; 1024: 155, 416 -> 138, 392.
-// NSHIP_MOE_SPLIT_MIN (a testing knob): the least slots an expert, of any size.
 bool split_takes(const MoeShape& m) {
   if (m.D <= 128 || m.H <= 128) return false;
   const int64_t N = m.T * m.K;
-  if (const char* knob = getenv("NSHIP_MOE_SPLIT_MIN")) return N >= std::max<int64_t>(1, atoll(knob)) * m.E;
+  if (const int64_t least = g_split_least.load(std::memory_order_relaxed)) return N >= least * m.E;
   const bool odd = m.D % 4 || m.H % 4;
   return N >= (odd ? 192 : 288) * m.E && (double)N * m.D * m.H >= (odd ? 0x1p28 : 6 * 0x1p30);
 }

@@ -2202,6 +2202,11 @@ int nsh_op_moe_experts_grad(const float* dy, const float* x, const float* weight
                              (hipStream_t)stream);
 }
 
+// For tests, and not in nship.h: from here on layers of D, H > 128 with `slots`
+// slots an expert take the pieces (0: by split_takes's own rule).  It decides what
+// sizes, states and workspaces mean, so a test sets it before it asks for them.
+void nsh_test_moe_split_least(int64_t slots) { set_split_least(slots); }
+
 // Sizes that the products' tiles and grids can index.
 static bool ns_shape_ok(int64_t n, int64_t r, int64_t c) {
   return n >= 0 && n <= 65535 && r >= 1 && c >= 1 && std::min(r, c) <= 32768 && std::max(r, c) <= (1 << 22) &&

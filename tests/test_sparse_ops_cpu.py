@@ -181,3 +181,28 @@ def test_newton_schulz_drives_the_singular_values():
         s = so.NS[0] * s + so.NS[1] * s ** 3 + so.NS[2] * s ** 5
     assert np.allclose(so.newton_schulz(g), (u * s) @ vt, atol=1e-12)
     assert np.allclose(so.newton_schulz(g.T), so.newton_schulz(g).T, atol=1e-13)
+
+
+@pytest.mark.parametrize("shape", [(400, 2, 200, 333, 4), (64, 2, 256, 256, 40), (3200, 2, 1024, 1024, 16)])
+def test_sizes_of_a_layer_do_not_hang_on_the_environment(shape, monkeypatch):
+    """A variable that changes between a sizing call and its launch, or between a
+    forward and its gradient, must not change what a buffer has to hold."""
+    lib = runtime.lib()
+    sizes = lambda: (lib.nsh_op_moe_experts_state(*shape), lib.nsh_op_moe_experts_workspace(*shape, 0),  # noqa: E731
+                     lib.nsh_op_moe_experts_workspace(*shape, 1))
+    before = sizes()
+    for value in ("1", "16", "100000"):
+        monkeypatch.setenv("NSHIP_MOE_SPLIT_MIN", value)
+        assert sizes() == before
+
+
+def test_a_tests_choice_of_the_pieces_ends_with_it():
+    lib = runtime.lib()
+    shape = (400, 2, 200, 333, 4)
+    before = lib.nsh_op_moe_experts_state(*shape)
+    try:
+        lib.nsh_test_moe_split_least(ctypes.c_int64(16))
+        assert lib.nsh_op_moe_experts_state(*shape) != before
+    finally:
+        lib.nsh_test_moe_split_least(ctypes.c_int64(0))
+    assert lib.nsh_op_moe_experts_state(*shape) == before
