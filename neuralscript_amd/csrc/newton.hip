@@ -351,22 +351,25 @@ __global__ __launch_bounds__(512) void ns_mid_kernel(NsArgs g) {
       for (int v = 0; v < 16; v++) part[wave - 4][q][v * 64 + lane] = acc[q >> 1][q & 1][v];
   }
   __syncthreads();
-  if (wave >= 4) return;
-  // (waves 4 .. 7 are gone: a barrier counts the four that are left)
+  if (wave < 4) {
 #pragma unroll
-  for (int q = 0; q < 4; q++)
+    for (int q = 0; q < 4; q++)
 #pragma unroll
-    for (int v = 0; v < 16; v++) {
-      acc[q >> 1][q & 1][v] += part[wave][q][v * 64 + lane];
-      part[wave][q][v * 64 + lane] = acc[q >> 1][q & 1][v];
-    }
+      for (int v = 0; v < 16; v++) {
+        acc[q >> 1][q & 1][v] += part[wave][q][v * 64 + lane];
+        part[wave][q][v * 64 + lane] = acc[q >> 1][q & 1][v];
+      }
+  }
   __syncthreads();
   floatx16 one[1][1];
+  if (wave < 4) {
 #pragma unroll
-  for (int v = 0; v < 16; v++)
-    one[0][0][v] = (part[0][wave][v * 64 + lane] + part[1][wave][v * 64 + lane]) +
-                   (part[2][wave][v * 64 + lane] + part[3][wave][v * 64 + lane]);
+    for (int v = 0; v < 16; v++)
+      one[0][0][v] = (part[0][wave][v * 64 + lane] + part[1][wave][v * 64 + lane]) +
+                     (part[2][wave][v * 64 + lane] + part[3][wave][v * 64 + lane]);
+  }
   __syncthreads();
+  if (wave >= 4) return;
   ns_epilogue<MODE, 1, 1>(g, one, reinterpret_cast<char*>(part) + wave * kTurnBytes, mat, mw + (wave >> 1) * 32,
                           nw + (wave & 1) * 32, l32, kh, kSym && tm == tn);
 }
