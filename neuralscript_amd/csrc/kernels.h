@@ -361,6 +361,8 @@ struct MuonNs {
   int nesterov;
 };
 size_t newton_schulz_bytes(int64_t n, int64_t r, int64_t c);
+void set_ns_tile_side(int side);  // (tests: see nsh_test_newton_tile)
+int ns_tile_side(int product, int64_t n, int64_t r, int64_t c);
 int launch_newton_schulz(const float* g, float* q, const MuonNs* step, int64_t n, int64_t r, int64_t c, int steps,
                          void* workspace, hipStream_t s);
 

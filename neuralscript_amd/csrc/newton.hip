@@ -25,6 +25,7 @@
 // ways, as the Gram product's operand (rows m, contraction N) and as the update's
 // (rows N, contraction m); S and P are symmetric and need one.
 #include <algorithm>
+#include <atomic>
 
 #include "common.h"
 #include "kernels.h"
@@ -814,39 +815,62 @@ struct NsSizes {
   }
 };
 
+// Tiles of `side` of n results [ra, rb] (sym: their lower triangles).
+int64_t tiles_of(int64_t n, int64_t ra, int64_t rb, int64_t side, bool sym) {
+  const int64_t tm = ceil_div(ra, side);
+  return n * (sym ? tm * (tm + 1) / 2 : tm * ceil_div(rb, side));
+}
+
+// Tests' choice of the tiles' side, also where one workgroup could take a matrix; 0: the rule.
+std::atomic<int> g_tile_side{0};
+
+// The side of a product's tiles, by the estimated us of each kernel from its
+// workgroups and K, as measured on 512 x 512, 4 of 512 x 512, 512 x 2048, 8192 x
+// 512, 2000 x 1500, 8 and 64 of 1024 x 1024: 32 x 32 outputs a workgroup 4 + 0.0031
+// K, or 2.2e-5 K each once they fill the chip; 64 x 64 6 + 0.0075 K, or 6.5e-5 K;
+// 128 x 128 9 + 0.0215 K on a CU by itself, 1.2 times as much for each of several;
+// 256 x 256 8 + 0.095 K.
+int tile_side(int64_t n, int64_t ra, int64_t rb, int64_t K, bool sym) {
+  if (const int side = g_tile_side.load(std::memory_order_relaxed)) return side;
+  const double k = (double)K;
+  const double t32 = (double)tiles_of(n, ra, rb, 32, sym), t64 = (double)tiles_of(n, ra, rb, 64, sym);
+  const int64_t n128 = ceil_div(tiles_of(n, ra, rb, 128, sym), 256), n256 = ceil_div(tiles_of(n, ra, rb, 256, sym), 256);
+  // (32 x 32 at most 2^22 workgroups: a launch takes fewer than 2^32 threads)
+  const double us[4] = {t32 > 0x1p22 ? 1e30 : std::max(4 + 0.0031 * k, 3 + 2.2e-5 * k * t32),
+                        std::max(6 + 0.0075 * k, 3 + 6.5e-5 * k * t64),
+                        9 + 0.0215 * k * (n128 == 1 ? 1. : 1.2 * n128), 8 + 0.095 * k * n256};
+  return 32 << (std::min_element(us, us + 4) - us);
+}
+
 template <int MODE>
 int launch_product(NsArgs& g, hipStream_t s) {
   constexpr bool kSym = MODE == kGram || MODE == kPoly;
-  auto tiles = [&](int64_t bm, int64_t bn) {
-    g.tiles_m = (int)ceil_div(g.ra, bm);
-    g.tiles_n = (int)ceil_div(g.rb, bn);
-    const int64_t t = kSym ? (int64_t)g.tiles_m * (g.tiles_m + 1) / 2 : (int64_t)g.tiles_m * g.tiles_n;
-    g.tiles = (int)t;
-    return t * g.n;
-  };
-  // Estimated us of each kernel from its workgroups and K, as measured on 512 x
-  // 512, 4 of 512 x 512, 512 x 2048, 8192 x 512, 2000 x 1500, 8 and 64 of 1024 x
-  // 1024: 32 x 32 outputs a workgroup 4 + 0.0031 K, or 2.2e-5 K each once they fill
-  // the chip; 64 x 64 6 + 0.0075 K, or 6.5e-5 K; 128 x 128 9 + 0.0215 K on a CU by
-  // itself, 1.2 times as much for each of several; 256 x 256 8 + 0.095 K.
-  const double k = (double)g.k;
-  const double t32 = (double)tiles(32, 32), t64 = (double)tiles(64, 64);
-  const int64_t n128 = ceil_div(tiles(128, 128), 256), n256 = ceil_div(tiles(256, 256), 256);
-  // (32 x 32 at most 2^22 workgroups: a launch takes fewer than 2^32 threads)
-  const double us[4] = {t32 > 0x1p22 ? 1e30 : std::max(4 + 0.0031 * k, 3 + 2.2e-5 * k * t32), std::max(6 + 0.0075 * k, 3 + 6.5e-5 * k * t64),
-                        9 + 0.0215 * k * (n128 == 1 ? 1. : 1.2 * n128), 8 + 0.095 * k * n256};
-  const int64_t side[4] = {32, 64, 128, 256};
-  const int use = (int)(std::min_element(us, us + 4) - us);
-  const dim3 grid((unsigned)tiles(side[use], side[use]));
-  if (use == 0) hipLaunchKernelGGL((ns_few_kernel<MODE>), grid, dim3(512), 0, s, g);
-  else if (use == 1) hipLaunchKernelGGL((ns_mid_kernel<MODE>), grid, dim3(512), 0, s, g);
-  else if (use == 2) hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 2, 2, 2, 32>), grid, dim3(256), 0, s, g);
+  const int side = tile_side(g.n, g.ra, g.rb, g.k, kSym);
+  g.tiles_m = (int)ceil_div(g.ra, side);
+  g.tiles_n = (int)ceil_div(g.rb, side);
+  g.tiles = (int)tiles_of(1, g.ra, g.rb, side, kSym);
+  const dim3 grid((unsigned)((int64_t)g.tiles * g.n));
+  if (side == 32) hipLaunchKernelGGL((ns_few_kernel<MODE>), grid, dim3(512), 0, s, g);
+  else if (side == 64) hipLaunchKernelGGL((ns_mid_kernel<MODE>), grid, dim3(512), 0, s, g);
+  else if (side == 128) hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 2, 2, 2, 32>), grid, dim3(256), 0, s, g);
   else hipLaunchKernelGGL((ns_gemm_kernel<MODE, 2, 4, 4, 2, 16>), grid, dim3(512), 0, s, g);
   NSH_LAUNCHED();
   return 0;
 }
 
 }  // namespace
+
+void set_ns_tile_side(int side) {
+  g_tile_side.store(side == 32 || side == 64 || side == 128 || side == 256 ? side : 0, std::memory_order_relaxed);
+}
+
+// 0: one workgroup a matrix; else the side of the tiles of the products S (0), P (1), X (2) and the last (3).
+int ns_tile_side(int product, int64_t n, int64_t r, int64_t c) {
+  const NsSizes z(r, c);
+  if (!g_tile_side.load(std::memory_order_relaxed) && ns_fused_fits(z.m, z.N)) return 0;
+  if (product < 2) return tile_side(n, z.m, z.m, product ? z.mp : z.np, true);
+  return product == 3 && r > c ? tile_side(n, z.N, z.m, z.mp, false) : tile_side(n, z.m, z.N, z.mp, false);
+}
 
 // the norms' partial sums; their exponents; X as the Gram's operand, twice as the update's; S and P
 size_t newton_schulz_bytes(int64_t n, int64_t r, int64_t c) {
@@ -870,7 +894,7 @@ int launch_newton_schulz(const float* g, float* q, const MuonNs* step, int64_t n
   float* mom = step ? step->m : nullptr;
   const float mu = step ? step->mu : 0.f;
   const int nesterov = step ? step->nesterov : 0;
-  if (steps > 0 && ns_fused_fits(z.m, z.N)) {
+  if (steps > 0 && ns_tile_side(0, n, r, c) == 0) {
     NsFused f{};
     f.g = g; f.m = mom; f.mu = mu; f.nesterov = nesterov;
     f.r = (int)r; f.c = (int)c; f.M = (int)z.m; f.N = (int)z.N;

@@ -2213,6 +2213,14 @@ static bool ns_shape_ok(int64_t n, int64_t r, int64_t c) {
          n * (ceil_div(r, 64) * ceil_div(c, 64)) <= (1 << 22);
 }
 
+// For tests, and not in nship.h: every product from here on by tiles of `side` (32,
+// 64, 128, 256; 0: by rule), and the side that a product (0 S, 1 P, 2 X, 3 the last
+// X) of n matrices [r, c] takes (0: one workgroup a matrix).
+void nsh_test_newton_tile(int side) { set_ns_tile_side(side); }
+int nsh_test_newton_side(int product, int64_t n, int64_t r, int64_t c) {
+  return ns_shape_ok(n, r, c) && n > 0 ? ns_tile_side(product, n, r, c) : -1;
+}
+
 size_t nsh_op_newton_schulz_workspace(int64_t n, int64_t r, int64_t c) {
   return ns_shape_ok(n, r, c) ? newton_schulz_bytes(n, r, c) : 0;
 }
