@@ -14,8 +14,15 @@
 // Products of two fp16 pieces (split2.h).  The map keeps |X| and |S| (entries and
 // singular values) below 1.21^2 and |P| below 3.45 whatever G is, so one power of
 // two per operand puts every entry into fp16's range.  Measured against 64 bits,
-// relative, fp32 products and these: 8 of 64 x 256 1.4e-6, 1.4e-6; 1000 x 333
-// 2.7e-6, 1.3e-6.
+// relative, fp32 products and these: 8 of 64 x 256 1.5e-6, 1.3e-6; 333 x 1000
+// 2.2e-6, 1.1e-6.
+//
+// One scale a matrix leaves the entries of a small row or column of G (an embedding's
+// row that few tokens read) far below it, so the low pieces are held times 2^11: an
+// entry of X keeps its 22 bits down to 2^-29, and below that an absolute 2^-51.
+// Relative errors of every third row of 512 x 2048 at 1e-4, 1e-6, 1e-8 of the others,
+// by themselves: 3.2e-7, 4.0e-7, 2.7e-5 (fp32 3.3e-7); with low pieces beside the high
+// ones 4.9e-6, 4.9e-4, 4.9e-2, for which the products of 64 of 1024 x 1024 took 4% less.
 //
 // The norm's 1e-7 leaves X0 small where G is.  X is then held times 2^e, e = e0 -
 // 2 k at step k and not below 0 (a step grows X by at most 3.4445), so that its
@@ -143,10 +150,10 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& g, const floatx16 (&ac
           for (int u = 0; u < 4; u++) {
             float x = acc[r][c][4 * q + u] * by;
             if (MODE == kPoly)
-              x += (k + u == col ? kNsA * kUpP : 0.f) + bs * ((float)sh[u] + (float)sl[u]);
+              x += (k + u == col ? kNsA * kUpP : 0.f) + bs * join2_far(sh[u], sl[u]);
             x = k + u < g.ra && col < g.rb ? x : 0.f;  // (padding)
             _Float16 hh, ll;
-            split2(x, hh, ll);
+            split2_far(x, hh, ll);
             h[u] = hh;
             l[u] = ll;
           }
@@ -185,7 +192,7 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& g, const floatx16 (&ac
 // One tile of C = A B^T (split2.h).
 template <int MODE, int WM, int WN, int TM, int TN, int KS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void ns_gemm_kernel(NsArgs g) {
-  using Tile = Split2Tile<WM, WN, TM, TN, KS>;
+  using Tile = Split2Tile<WM, WN, TM, TN, KS, true>;
   static_assert(kTurnBytes * WM * WN <= Tile::kLds, "the transposing tiles fit");
   constexpr bool kSym = MODE == kGram || MODE == kPoly;
   static_assert(!kSym || Tile::RA == Tile::RB, "a symmetric result's tiles are square");
@@ -224,9 +231,9 @@ __global__ __launch_bounds__(512) void ns_few_kernel(NsArgs g) {
   int tm, tn;
   ns_tile<kSym>(L % g.tiles, g.tiles_n, tm, tn);
   const int64_t mw = (int64_t)tm * 32, nw = (int64_t)tn * 32;
-  floatx16 acc;
+  floatx16 acc, low;
 #pragma unroll
-  for (int v = 0; v < 16; v++) acc[v] = 0.f;
+  for (int v = 0; v < 16; v++) acc[v] = low[v] = 0.f;
   {
     // chunk (piece, octet 2 s + kh, row) of step s
     const half8* pa = reinterpret_cast<const half8*>(g.A + mat * g.sA) + kh * g.ra + min(mw + l32, g.ra - 1);
@@ -248,9 +255,9 @@ __global__ __launch_bounds__(512) void ns_few_kernel(NsArgs g) {
       __builtin_amdgcn_sched_barrier(0);  // (all loads first)
 #pragma unroll
       for (int u = 0; u < CNT; u++) {
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][1], b[u][0], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][0], b[u][1], acc, 0, 0, 0);
+        low = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][1], b[u][0], low, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][0], b[u][0], acc, 0, 0, 0);
+        low = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][0], b[u][1], low, 0, 0, 0);
       }
     };
     int s = wave;
@@ -265,6 +272,8 @@ __global__ __launch_bounds__(512) void ns_few_kernel(NsArgs g) {
     }
     if (s < all) steps(s, std::integral_constant<int, 1>{});
   }
+#pragma unroll
+  for (int v = 0; v < 16; v++) acc[v] += kLowDown * low[v];
   if (wave > 0) {
 #pragma unroll
     for (int v = 0; v < 16; v++) part[wave - 1][v * 64 + lane] = acc[v];
@@ -284,7 +293,7 @@ __global__ __launch_bounds__(512) void ns_few_kernel(NsArgs g) {
 // with the whole tile over its share of K (half of the loads a product that 32 x
 // 32 outputs take), the eight sums met in LDS, where wave (i, j) of the first four
 // takes its block's.
-constexpr int kMidU = 3;
+constexpr int kMidU = 2;
 template <int MODE>
 __global__ __launch_bounds__(512) void ns_mid_kernel(NsArgs g) {
   constexpr bool kSym = MODE == kGram || MODE == kPoly;
@@ -296,13 +305,13 @@ __global__ __launch_bounds__(512) void ns_mid_kernel(NsArgs g) {
   int tm, tn;
   ns_tile<kSym>(L % g.tiles, g.tiles_n, tm, tn);
   const int64_t mw = (int64_t)tm * 64, nw = (int64_t)tn * 64;
-  floatx16 acc[2][2];
+  floatx16 acc[2][2], low[2][2];
 #pragma unroll
   for (int i = 0; i < 2; i++)
 #pragma unroll
     for (int j = 0; j < 2; j++)
 #pragma unroll
-      for (int v = 0; v < 16; v++) acc[i][j][v] = 0.f;
+      for (int v = 0; v < 16; v++) acc[i][j][v] = low[i][j][v] = 0.f;
   {
     const half8 *pa[2], *pb[2];
 #pragma unroll
@@ -330,21 +339,25 @@ __global__ __launch_bounds__(512) void ns_mid_kernel(NsArgs g) {
 #pragma unroll
       for (int u = 0; u < CNT; u++)
 #pragma unroll
-        for (int q = 0; q < 3; q++)  // l h, h l, h h
+        for (int q = 0; q < 3; q++)  // l h, h h, h l
 #pragma unroll
           for (int i = 0; i < 2; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][i][q == 0], b[u][j][q == 1], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < 2; j++) {
+              floatx16& to = q == 1 ? acc[i][j] : low[i][j];
+              to = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u][i][q == 0], b[u][j][q == 2], to, 0, 0, 0);
+            }
     };
     int s = wave;
     for (; s + 8 * (kMidU - 1) < all; s += 8 * kMidU) steps(s, std::integral_constant<int, kMidU>{});
-    if (s + 8 < all) {
-      steps(s, std::integral_constant<int, 2>{});
-      s += 16;
-    }
     if (s < all) steps(s, std::integral_constant<int, 1>{});
   }
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) acc[i][j][v] += kLowDown * low[i][j][v];
   if (wave >= 4) {
 #pragma unroll
     for (int q = 0; q < 4; q++)
@@ -487,7 +500,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(NsStart a) {
 #pragma unroll
       for (int u = 0; u < 8; u++) {
         _Float16 hh, ll;
-        split2(x[lo][8 * o + u], hh, ll);
+        split2_far(x[lo][8 * o + u], hh, ll);
         h[u] = hh;
         l[u] = ll;
       }
@@ -499,7 +512,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(NsStart a) {
 #pragma unroll
       for (int u = 0; u < 8; u++) {
         _Float16 hh, ll;
-        split2(x[8 * o + u][lo], hh, ll);
+        split2_far(x[8 * o + u][lo], hh, ll);
         h[u] = hh;
         l[u] = ll;
       }
@@ -532,7 +545,7 @@ __global__ __launch_bounds__(256) void ns_normalise_kernel(const float* g, const
 // spread over the banks): up to 64 x 256.  A step is three products with a barrier
 // between: S and P in 16 x 16 blocks (of 32 x 32 most waves would have none), X in
 // 32 x 32 ones (half of the LDS reads).  Bound by LDS traffic and the waves'
-// latency: 8 of 64 x 256 in 5 steps 35 us (84 with a launch for each product).
+// latency: 8 of 64 x 256 in 5 steps 36 us (84 with a launch for each product).
 constexpr int kNsLds = 163840;
 struct NsFused {
   const float* g;
@@ -621,7 +634,7 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
 #pragma unroll
     for (int u = 0; u < 8; u++) {
       _Float16 hh, ll;
-      split2(8 * o + u < ks ? (float)(v[u] * up) : 0.f, hh, ll);
+      split2_far(8 * o + u < ks ? (float)(v[u] * up) : 0.f, hh, ll);
       h[u] = hh;
       l[u] = ll;
     }
@@ -666,7 +679,7 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
       lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, b0, lo, 0, 0, 0);
       lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b1, lo, 0, 0, 0);
     }
-    return hi + lo;
+    return hi + kLowDown * lo;
   };
   // its values into S's or P's operand, both ways unless on the diagonal
   auto put16 = [&](const floatx4& x, int bi, int bj) {
@@ -675,7 +688,7 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       _Float16 hh, ll;
-      split2(x[u], hh, ll);
+      split2_far(x[u], hh, ll);
       h[u] = hh;
       l[u] = ll;
       if (bi != bj) {
@@ -708,8 +721,8 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
         for (int v = 0; v < 4; v++) {
           // (as P's square sees it: a rounding of S in one term alone would reach P four times as large)
           _Float16 h, l;
-          split2(S[q][v] * (kUpS / (kUpX * kUpX)), h, l);
-          S[q][v] = (float)h + (float)l;
+          split2_far(S[q][v] * (kUpS / (kUpX * kUpX)), h, l);
+          S[q][v] = join2_far(h, l);
         }
         put16(S[q], si[q], sj[q]);
       }
@@ -731,7 +744,7 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
       if (wave + kW * q < tri) put16(S[q], si[q], sj[q]);
     __syncthreads();
     // X: 32 x 32 block (b / nb, b % nb) of P X over the 16-steps of m
-    floatx16 x[kBlocks];
+    floatx16 x[kBlocks], low;
 #pragma unroll
     for (int q = 0; q < kBlocks; q++) {
       const int b = wave + kW * q;
@@ -740,14 +753,16 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
         const half8* pa = reinterpret_cast<const half8*>(sym) + kh * rm + b / nb * 32 + l32;
         const half8* pb = reinterpret_cast<const half8*>(upd) + kh * rn + b % nb * 32 + l32;
 #pragma unroll
-        for (int v = 0; v < 16; v++) x[q][v] = 0.f;
+        for (int v = 0; v < 16; v++) x[q][v] = low[v] = 0.f;
 #pragma unroll 4
         for (int s = 0; s < mp / 16; s++) {
           const half8 a0 = pa[2 * s * rm], a1 = pa[2 * s * rm + ps / 8], b0 = pb[2 * s * rn], b1 = pb[2 * s * rn + pu / 8];
-          x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b0, x[q], 0, 0, 0);
-          x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b1, x[q], 0, 0, 0);
+          low = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b0, low, 0, 0, 0);
           x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b0, x[q], 0, 0, 0);
+          low = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b1, low, 0, 0, 0);
         }
+#pragma unroll
+        for (int v = 0; v < 16; v++) x[q][v] += kLowDown * low[v];
       }
     }
     const bool last = step + 1 == a.steps;
@@ -777,7 +792,7 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
           _Float16 hh, ll;
-          split2(x[q][4 * w + u] * xs, hh, ll);
+          split2_far(x[q][4 * w + u] * xs, hh, ll);
           h[u] = hh;
           l[u] = ll;
           _Float16* p = gram + ((col >> 3) * rm + row0 + 8 * w + u) * 8 + (col & 7);
@@ -828,8 +843,9 @@ std::atomic<int> g_tile_side{0};
 // workgroups and K, as measured on 512 x 512, 4 of 512 x 512, 512 x 2048, 8192 x
 // 512, 2000 x 1500, 8 and 64 of 1024 x 1024: 32 x 32 outputs a workgroup 4 + 0.0031
 // K, or 2.2e-5 K each once they fill the chip; 64 x 64 6 + 0.0075 K, or 6.5e-5 K;
-// 128 x 128 9 + 0.0215 K on a CU by itself, 1.2 times as much for each of several;
-// 256 x 256 8 + 0.095 K.
+// 128 x 128 9 + 0.0215 K on a CU by itself, 1.3 times as much for each of several;
+// 256 x 256 8 + 0.107 K.  X of 64 of 1024 x 1024: 1700, 850, 462, 446 us; of 512 x
+// 2048: 20, 11, 21, 48; S of 512 x 512: 6, 9.5, 18, 44.
 int tile_side(int64_t n, int64_t ra, int64_t rb, int64_t K, bool sym) {
   if (const int side = g_tile_side.load(std::memory_order_relaxed)) return side;
   const double k = (double)K;
@@ -838,7 +854,7 @@ int tile_side(int64_t n, int64_t ra, int64_t rb, int64_t K, bool sym) {
   // (32 x 32 at most 2^22 workgroups: a launch takes fewer than 2^32 threads)
   const double us[4] = {t32 > 0x1p22 ? 1e30 : std::max(4 + 0.0031 * k, 3 + 2.2e-5 * k * t32),
                         std::max(6 + 0.0075 * k, 3 + 6.5e-5 * k * t64),
-                        9 + 0.0215 * k * (n128 == 1 ? 1. : 1.2 * n128), 8 + 0.095 * k * n256};
+                        9 + 0.0215 * k * (n128 == 1 ? 1. : 1.3 * n128), 8 + 0.107 * k * n256};
   return 32 << (std::min_element(us, us + 4) - us);
 }
 

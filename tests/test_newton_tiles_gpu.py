@@ -92,3 +92,41 @@ def test_newton_schulz_by_the_rule(n, r, c):
     for i in range(min(n, 2)):
         close(out[i], g[i], f"matrix {i}", 2)
     assert all(np.array_equal(out[i], out[0]) for i in range(3, n))
+
+
+def close_by_rows(got, g, what):
+    """Each row by itself: four times fp32's error and 16 U, as close() allows, and
+    what entries below fp16's normal range lose.  With m <= N and rho the row's share
+    of |G|_F: an entry of X or S is off by at most e = 2^-51, of P by 2 e, so a step
+    leaves a row's S off by 1.21 e sqrt(N) + e sqrt(m), its P by 2 e sqrt(m) + 10.7 times
+    that (4.775 + 2 2.0315 1.21^2 of it), and X by 1.21 times P's and 3.45 e sqrt(N):
+    35 e sqrt(N) in all, of a row that starts at rho and that no step makes
+    smaller than by 0.68: 5 steps' are below 2^8 e sqrt(N) / rho."""
+    want, fp32 = so.newton_schulz(g), so.newton_schulz(g, 5, np.float32)
+    size = np.linalg.norm(want, axis=1)
+    rho = np.linalg.norm(g.astype(np.float64), axis=1) / np.linalg.norm(g.astype(np.float64))
+    off = np.linalg.norm(got - want, axis=1)
+    allowed = 4 * np.linalg.norm(fp32 - want, axis=1) + (16 * U + 2.0 ** -43 * np.sqrt(max(g.shape)) / rho) * size
+    print(f"  {what}: rows off by {(off / size).max():.3g}, {(off / allowed).max():.3g} of the bound", flush=True)
+    assert np.all(off <= allowed), what
+
+
+def small_rows(r, c, scale, seed):
+    g = np.random.default_rng(seed).normal(size=(1, r, c)).astype(np.float32)
+    g[:, ::3] *= np.float32(scale)
+    return g
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1e-4, 1e-5, 1e-6])
+@pytest.mark.parametrize("r,c", [(130, 300), (300, 130), (257, 257)])
+def test_small_rows_keep_their_own_accuracy_by_tiles(r, c, scale, side):
+    """Rows of an embedding that few tokens read."""
+    g = small_rows(r, c, scale, r)
+    close_by_rows(run_ns(g)[0], g[0], f"{r} x {c}, {scale:g}, tiles of {side}")
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1e-4, 1e-5, 1e-6])
+@pytest.mark.parametrize("r,c", [(64, 256), (256, 64), (90, 90), (512, 2048), (2048, 512)])
+def test_small_rows_keep_their_own_accuracy(r, c, scale):
+    g = small_rows(r, c, scale, c)
+    close_by_rows(run_ns(g)[0], g[0], f"{r} x {c}, {scale:g}")
