@@ -97,7 +97,6 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& g, const floatx16 (&ac
   const int ex = max(0, g.ex[mat] - 2 * g.step);  // X = 2^-ex times what is held
   if constexpr (MODE == kLast) {
     float* __restrict__ f = g.f + mat * g.ra * g.rb;
-    const float down = ldexpf(1.f / (kUpX * kUpP), -ex);
 #pragma unroll
     for (int r = 0; r < TM; r++)
 #pragma unroll
@@ -114,7 +113,8 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& g, const floatx16 (&ac
 #pragma unroll
         for (int v = 0; v < 16; v++) {
           const int dr = 8 * (v >> 2) + (v & 3);
-          const float x = acc[r][c][v] * down;
+          // (not times 2^-ex 2^-29, which underflows where X still does not)
+          const float x = ldexpf(acc[r][c][v] * (1.f / (kUpX * kUpP)), -ex);
           if (row0 + dr < g.ra) p[dr * g.rb] = g.weights ? w[v] - g.le * x - g.decay * w[v] : x;
         }
       }
@@ -766,7 +766,7 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
       }
     }
     const bool last = step + 1 == a.steps;
-    const float xs = last ? ldexpf(1.f / (kUpX * kUpP), -ex) : ldexpf(1.f / kUpP, max(0, ex - 2) - ex);
+    const float xs = last ? 1.f / (kUpX * kUpP) : ldexpf(1.f / kUpP, max(0, ex - 2) - ex);
     if (!last) __syncthreads();
 #pragma unroll
     for (int q = 0; q < kBlocks; q++) {
@@ -780,7 +780,7 @@ __global__ __launch_bounds__(1024) void ns_fused_kernel(NsFused a) {
           const int i = row0 + 8 * (v >> 2) + (v & 3);
           if (i >= a.M || col >= a.N) continue;
           float* p = a.f + base + (tall ? col * a.c + i : i * a.c + col);
-          const float y = x[q][v] * xs;
+          const float y = ldexpf(x[q][v] * xs, -ex);
           *p = a.weights ? *p - a.le * y - a.decay * *p : y;
         }
         continue;

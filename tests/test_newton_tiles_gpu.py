@@ -130,3 +130,23 @@ def test_small_rows_keep_their_own_accuracy_by_tiles(r, c, scale, side):
 def test_small_rows_keep_their_own_accuracy(r, c, scale):
     g = small_rows(r, c, scale, c)
     close_by_rows(run_ns(g)[0], g[0], f"{r} x {c}, {scale:g}")
+
+
+@pytest.mark.parametrize("r,c,by", [(40, 72, 0), (72, 40, 0), (40, 72, 32), (72, 40, 64), (140, 72, 128), (72, 140, 256)])
+@pytest.mark.parametrize("steps", [1, 2, 3, 5])
+def test_the_smallest_gradients(r, c, by, steps):
+    """A gradient of a few of fp32's smallest values: its norm is far below the 1e-7
+    beside it, and a few steps leave X small, but within fp32's normal range.  One
+    entry a row and column, so each is scaled by 3.4445^steps / 1e-7 up to rounding:
+    16 U, and the 2 U of a norm next to 1e-7."""
+    g = np.zeros((1, r, c), np.float32)
+    for i in range(3):
+        g[0, 7 * i, 11 * i] = (-1) ** i * (i + 3) * 1.4013e-45
+    runtime.lib().nsh_test_newton_tile(by)
+    try:
+        got = run_ns(g, steps)[0].astype(np.float64)
+    finally:
+        runtime.lib().nsh_test_newton_tile(0)
+    want = g[0].astype(np.float64) / 1e-7 * so.NS[0] ** steps
+    assert np.abs(want[want != 0]).min() > 1.2e-38
+    assert np.all(np.abs(got - want) <= 18 * steps * U * np.abs(want))
