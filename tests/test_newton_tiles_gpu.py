@@ -9,7 +9,9 @@ import pytest
 import sparse_oracle as so
 from neuralscript_amd import runtime
 from sparse_oracle import U, p, put, room
+from test_moe_branches_gpu import repeated, window
 from test_newton_schulz_gpu import close, run_ns
+from test_sparse_large_gpu import Plain, room_for
 
 pytestmark = pytest.mark.gpu
 i64 = ctypes.c_int64
@@ -150,3 +152,22 @@ def test_the_smallest_gradients(r, c, by, steps):
     want = g[0].astype(np.float64) / 1e-7 * so.NS[0] ** steps
     assert np.abs(want[want != 0]).min() > 1.2e-38
     assert np.all(np.abs(got - want) <= 18 * steps * U * np.abs(want))
+
+
+def test_matrices_beyond_32_bits():
+    """2^31 entries and more, in place: four matrices over and over."""
+    n, r, c = 2052, 1024, 1032
+    g = np.random.default_rng(3).normal(size=(4, r, c)).astype(np.float32)
+    ws = runtime.lib().nsh_op_newton_schulz_workspace(n, r, c)
+    assert n * r * c > 1 << 31
+    room_for(ws + 4 * n * r * c + (1 << 30))
+    d, room_ = repeated(g, n // 4), Plain(ws, 0xFF)
+    runtime.op("newton_schulz", d.ptr, d.ptr, n, r, c, 1, room_.ptr, None)
+    so.sync()
+    first = window(d, 0, g.shape)
+    for i in range(2):
+        close(first[i], g[i], f"matrix {i}", 1)
+    for at in (n // 8 * 4, n - 4):  # (whole periods)
+        assert np.array_equal(window(d, at, g.shape), first)
+    d.free()
+    room_.free()
