@@ -279,8 +279,8 @@ int nsh_op_moe_route(const float* logits, const float* bias, const uint8_t* acti
 /* The gradient of nsh_op_moe_route's weights: dlogits [T, E] from dweight
  * [T, K], the choice (idx; the bias and the groups act through it alone) and
  * the same logits, active, score, renorm and scale.  dweight of a slot whose
- * idx is out of range or not live is not read; dlogits is 0 where an expert is
- * not live.  Weights that are 0 because all scores underflowed in 64 bits have a
+ * idx is out of range or not live counts for nothing, whatever it holds; dlogits
+ * is 0 where an expert is not live.  Weights that are 0 because all scores underflowed in 64 bits have a
  * gradient of 0. */
 int nsh_op_moe_route_grad(const float* dweight, const float* logits, const uint8_t* active, const int32_t* idx,
                           float* dlogits, int64_t T, int64_t E, int64_t K, int score, int renorm, float scale,
