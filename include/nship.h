@@ -321,10 +321,10 @@ int nsh_op_moe_experts_grad(const float* dy, const float* x, const float* weight
  * g, q [n, r, c]; q may be g.  A matrix with an infinity or NaN comes out as
  * NaN, a zero one as zeros; the others of the batch are not touched by it.
  * Accuracy: fp32 sums of products whose operands are held to 22 bits of each
- * entry, under one scale a matrix: an entry of X below 2^-29 (of A below 2^-29, of
- * the polynomial below 2^-28) to an absolute 2^-51 (2^-51, 2^-50).  The error is that
- * of fp32 or less, also in a row of G by itself, down to rows at 1e-6 of |G|_F /
- * sqrt(min(r, c)); at 1e-8 of it 3e-5 of the row.
+ * entry, under one scale a matrix: an entry of X or A below 2^-29 to an absolute
+ * 2^-51, of the polynomial below 2^-28 to 2^-50.  The error is that of fp32 or less,
+ * also in a row or column of G by itself whose entries are above 2^-29 |G|_F: of 512
+ * x 2048, rows at 1e-6 of the others (4e-7); those at 1e-8 come out 3e-5 off.
  * n <= 65535, min(r, c) <= 32768, max(r, c) <= 2^22, and n matrices of at most
  * 2^22 blocks of 64 x 64 together. */
 size_t nsh_op_newton_schulz_workspace(int64_t n, int64_t r, int64_t c);
