@@ -295,8 +295,9 @@ int nsh_op_moe_route_grad(const float* dweight, const float* logits, const uint8
  * products' operands as 22 bits of each entry, down to 2^-17 of a scale, and
  * below that as an absolute 2^-40 of it: the largest entry of the slot's row of x
  * or dy and of the expert matrix's row or column that is summed over; for act(u)
- * and du the product of the two operands' 2-norms; in the weights' gradients the
- * largest of these over the expert's slots.  Other layers take 24 bits.
+ * and du the product of the two operands' 2-norms.  In the weights' gradients the
+ * scale is the largest of these over the expert's slots, and the entries keep 22
+ * bits down to 2^-28 of it and an absolute 2^-51 below.  Other layers take 24 bits.
  * state (NULL for inference): keeps what the gradient needs. */
 size_t nsh_op_moe_experts_state(int64_t T, int64_t K, int64_t D, int64_t H, int64_t E);
 size_t nsh_op_moe_experts_workspace(int64_t T, int64_t K, int64_t D, int64_t H, int64_t E, int grad);

@@ -21,7 +21,13 @@
 // written as pieces by the epilogue that makes them, before their largest entry
 // is known: their scale is the Cauchy-Schwarz bound |x| max |W1 column| (2-norms,
 // rounded up to powers of two), some 2^4 above the largest entry.  Where
-// positions are the contraction, one scale serves an expert's segment.
+// positions are the contraction, one scale serves an expert's segment, with the
+// features and hidden units far below its largest: there the low pieces are held
+// times 2^11 (split2.h), 22 bits down to 2^-28 and an absolute 2^-51 below.  Relative
+// errors of the rows and columns of the weights' gradients of units at 1e-4, 1e-6
+// and 1e-8 of the others, by themselves, 500 tokens of 136 x 160: 2.7e-7, 2.7e-7,
+// 1.0e-5 (three pieces 3e-7); with low pieces beside the high ones 2.0e-6, 1.8e-4,
+// 1.9e-2, in 1.6% less of a training step.
 //
 // Passes beside the products: the weights' layouts (read twice, written once),
 // x and dy gathered by position, and for the gradient both once more with
@@ -41,17 +47,23 @@ namespace {
 // other's products.  131072 slots of 64 experts of 1024 x 1024, us, hidden and slots
 // products: 1172, 949 (235 and 290 TFLOP/s); 256 x 256, one workgroup of eight waves
 // on a CU: 1308, 1050.
-constexpr int kTM = 4, kTN = 2, kWM = 2, kWN = 2, kWaves = kWM * kWN;
-using Tile = Split2Tile<kWM, kWN, kTM, kTN, 16>;
+// The weights' gradients have accumulators for the products with a low piece beside
+// the others, and eight waves of half the blocks: 16384 tokens, 2 of 64 experts of
+// 1024 x 1024, 273 us a product (290 with the two sums in turn on the waves above,
+// 253 with one sum).
+constexpr int kWN = 2, kTN = 2;
+using Tile = Split2Tile<2, kWN, 4, kTN, 16>;
+using FarTile = Split2Tile<4, kWN, 2, kTN, 16, true>;  // the weights' gradients
 constexpr int kPad = 32;      // positions a segment is padded to
 constexpr int kNoExp = -300;  // "the logarithm of 0"
 constexpr int kPitch = 40;    // halves of a transposing tile's row
 constexpr int kTurnBytes = 2 * 32 * kPitch * 2;
 
-// v = h + l, with l = 0 beside an infinite h (not inf - inf).
+// v = h + l (FAR: h + 2^-11 l, split2.h), with l = 0 beside an infinite h (not inf - inf).
+template <bool FAR = false>
 __device__ __forceinline__ void split2_any(float v, _Float16& h, _Float16& l) {
   h = (_Float16)v;
-  const float r = v - (float)h;
+  const float r = (v - (float)h) * (FAR ? kLowUp : 1.f);
   l = (_Float16)(fabsf(v) > 65504.f ? 0.f : r);
 }
 __device__ __forceinline__ float finite_abs(float v) {
@@ -70,12 +82,13 @@ __device__ __forceinline__ int row_exp(float top) { return top > 0.f ? 14 - ilog
 __device__ __forceinline__ int seg_exp(int top) { return top > kNoExp ? -top : 0; }
 __device__ __forceinline__ int log2_norm(double sq) { return sq > 0. ? log2_up(sqrt(sq)) : kNoExp; }
 
+template <bool FAR = false>
 __device__ __forceinline__ void put_chunk(_Float16* __restrict__ to, int64_t piece, const float (&v)[8]) {
   half8 h, l;
 #pragma unroll
   for (int u = 0; u < 8; u++) {
     _Float16 hh, ll;
-    split2_any(v[u], hh, ll);
+    split2_any<FAR>(v[u], hh, ll);
     h[u] = hh;
     l[u] = ll;
   }
@@ -320,7 +333,7 @@ __global__ __launch_bounds__(256) void turn_kernel(const float* __restrict__ src
     const float f = src[(int64_t)(t < 0 ? 0 : t) * C + col];
     v[u] = t < 0 ? 0.f : ldexpf(f, ex);
   }
-  put_chunk(out + ((p0 / 8 + o) * C + col) * 8, np * C, v);
+  put_chunk<true>(out + ((p0 / 8 + o) * C + col) * 8, np * C, v);
 }
 
 // xw[e] = the largest log2 of |weight| times the bound of |act(u)|'s factor by
@@ -402,8 +415,11 @@ __device__ __forceinline__ int hidden_seg_exp(const SplitArgs& g, int e) {
   return b > kNoExp ? 15 - b : 0;
 }
 
+constexpr int waves_of(int mode) { return mode == kWeight ? FarTile::NT / 64 : Tile::NT / 64; }
+
 template <int MODE>
-__global__ __launch_bounds__(64 * kWaves, 2) void split_kernel(SplitArgs g) {
+__global__ __launch_bounds__(waves_of(MODE) * 64, 2) void split_kernel(SplitArgs g) {
+  constexpr int kWaves = waves_of(MODE), kTM = 16 / kWaves;
   static_assert(kTurnBytes * kWaves + 4 * Tile::RA <= Tile::kLds, "the transposing tiles and the exponents fit");
   __shared__ __attribute__((aligned(16))) char smem[Tile::kLds];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / kWN, wn = wave % kWN;
@@ -451,7 +467,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void split_kernel(SplitArgs g) {
                           arow + m0, arow + g.M - 1};
     const Split2Operand B{reinterpret_cast<const uintx4*>(g.B) + kbeg / 8 * g.brows, g.brows, g.kp / 8 * g.brows, n0,
                           nend - 1};
-    Tile::run(A, B, nk, smem, acc);
+    std::conditional_t<MODE == kWeight, FarTile, Tile>::run(A, B, nk, smem, acc);
   }
   const int64_t mw = m0 + wm * kTM * 32, nw = n0 + wn * kTN * 32;
   if constexpr (MODE == kWeight) {
@@ -583,10 +599,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void split_kernel(SplitArgs g) {
               l[u] = ll;
               // with positions as k: du now, weight act(u) after it
               _Float16* to = reinterpret_cast<_Float16*>(turn) + (8 * q + 4 * kh + u) * kPitch + l32;
-              split2_any(ok ? ldexpf(du, se1) : 0.f, hh, ll);
+              split2_any<true>(ok ? ldexpf(du, se1) : 0.f, hh, ll);
               to[0] = hh;
               to[32 * kPitch] = ll;
-              split2_any(ok ? ldexpf(hw, se2) : 0.f, hh, ll);
+              split2_any<true>(ok ? ldexpf(hw, se2) : 0.f, hh, ll);
               th[q][u] = hh;
               tl[q][u] = ll;
             }
@@ -742,11 +758,11 @@ void set_split_least(int64_t slots) { g_split_least.store(std::max<int64_t>(0, s
 // Both products on pieces cost the layouts of the weights (24 bytes an element,
 // forward) and some 50 us of passes, and save half of the products' time.  Sorted
 // fp32 operands -> this, us, forward and training step: 64 experts of 1024 x 1024,
-// slots an expert 192: 438, 1426 -> 501, 1461; 256: 598, 1879 -> 636, 1827; 384:
-// 808, 2559 -> 740, 2162; 1024: 1835, 5924 -> 1391, 4178.  16 of 512 x 2048, 384:
-// 298, 839 -> 292, 807.  8 of 256 x 256, 1024: 85, 222 -> 133, 357.  Where a size is
-// no multiple of 4 the others read it float by float: 10 of 200 x 333, 96: 118, 282
-// -> 117, 300; 192: 124, 323 -> 121, 317; 1024: 155, 416 -> 138, 392.
+// slots an expert 192: 473, 1423 -> 511, 1521; 256: 611, 1861 -> 646, 1864; 384:
+// 813, 2519 -> 756, 2221; 1024: 1839, 5948 -> 1407, 4327.  16 of 512 x 2048, 384:
+// 307, 854 -> 296, 840.  8 of 256 x 256, 1024: 74, 219 -> 136, 359.  Where a size is
+// no multiple of 4 the others read it float by float: 10 of 200 x 333, 96: 123, 288
+// -> 122, 303; 192: 130, 328 -> 125, 317; 1024: 159, 420 -> 143, 388.
 bool split_takes(const MoeShape& m) {
   if (m.D <= 128 || m.H <= 128) return false;
   const int64_t N = m.T * m.K;
@@ -836,7 +852,7 @@ static SplitArgs split_args(const MoeShape& m, const State& st, int64_t M, int a
 template <int MODE>
 static int split_product(const SplitArgs& g, int64_t entries, hipStream_t s) {
   hipLaunchKernelGGL(split_kernel<MODE>, dim3((unsigned)(entries * g.mt * (MODE == kWeight ? g.nt : 1))),
-                     dim3(64 * kWaves), 0, s, g);
+                     dim3(64 * waves_of(MODE)), 0, s, g);
   NSH_LAUNCHED();
   return 0;
 }

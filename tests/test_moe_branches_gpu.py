@@ -67,6 +67,32 @@ def test_experts_of_wide_layers_on_pieces(T, K, D, H, E, shift, pieces):
     check(layer(T, K, D, H, E, D, 0.05), 6, shift)
 
 
+# features of x, hidden units by either matrix, far smaller than the others
+@pytest.mark.parametrize("scale", [1e-4, 1e-6])
+@pytest.mark.parametrize("small", ["features", "units by W1", "units by W2", "tokens"])
+@pytest.mark.parametrize("act", [0, 6])
+def test_small_rows_of_the_weights_gradients_keep_their_own_accuracy(scale, small, act, pieces):
+    """Rows and columns of dW1 and dW2 by themselves, within what within() allows a
+    whole gradient: one scale serves all positions of an expert there."""
+    a = layer(500, 2, 136, 160, 2, 12)
+    if small == "features":
+        a["x"][:, ::3] *= np.float32(scale)
+    elif small == "units by W1":
+        a["W1"][:, :, ::3] *= np.float32(scale)
+    elif small == "units by W2":
+        a["W2"][:, ::3] *= np.float32(scale)
+    else:
+        a["x"][::3] *= np.float32(scale)
+        a["dy"][::3] *= np.float32(scale)
+    want, _ = so.experts(a["x"], a["idx"], a["weight"], a["W1"], a["W2"], act, a["dy"])
+    got = run_experts(a, 2, act, True)
+    for k in ("dW1", "dW2"):
+        for axis in (1, 2):
+            err = np.linalg.norm(got[k] - want[k], axis=axis) / np.linalg.norm(want[k], axis=axis)
+            print(f"  {k} along {axis}: {err.max():.3g}", flush=True)
+            assert np.all(err <= 1e-5), (k, axis)
+
+
 # without a sort: contractions of several stages (512 forward, 1024 backward), by
 # slots and by experts, more than 8 rows an expert, up to 1024 slots
 @pytest.mark.parametrize("T,K,D,H,E,skew", [(3, 2, 1030, 2100, 8, 0.0), (8, 2, 1028, 2052, 8, 0.0), (8, 2, 2051, 1025, 4, 0.5),
