@@ -26,7 +26,7 @@ typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 // The low piece times 2^11: it then lies in the high one's range, and v keeps its
 // 22 bits down to fp16's smallest normal, 2^-30 of its largest; below, an absolute
-// 2^-36.  For operands whose rows lie far apart under one scale (newton.hip).
+// 2^-36.  For operands whose rows lie far apart under one scale (newton.hip, moe_split.hip).
 constexpr float kLowUp = 0x1p11f, kLowDown = 0x1p-11f;
 __device__ __forceinline__ void split2_far(float v, _Float16& h, _Float16& l) {
   h = (_Float16)v;

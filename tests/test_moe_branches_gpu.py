@@ -2,6 +2,7 @@
 sort blocks and experts, contractions above 1024, several passes over a list,
 offsets beyond 32 bits; against the 64-bit formulas (sparse_oracle.py)."""
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -10,6 +11,7 @@ import sparse_oracle as so
 from neuralscript_amd import runtime
 from sparse_oracle import U, p, put
 from test_moe_topk_gpu import layer, run_experts, within
+from test_newton_schulz_gpu import Layer
 from test_sparse_large_gpu import Plain, room_for
 
 pytestmark = pytest.mark.gpu
@@ -166,3 +168,28 @@ def test_experts_beyond_32_bits(T, D, H, E):
         assert err <= np.sqrt(T / E) * U
     for b in (*d.values(), *out.values(), st, room):
         b.free()
+
+
+def test_two_host_threads_at_once(pieces):
+    """Training steps of layers that go other ways, each from a thread of its own on
+    a stream of its own: the bits of the same steps after each other."""
+    sizes = [(96, 2, 64, 96, 5), (12, 3, 36, 20, 4), (200, 2, 136, 260, 5)]
+
+    def steps(a, stream):
+        for _ in range(20):
+            a.step(stream)
+        so.sync(stream)
+
+    streams = [so.new_stream() for _ in sizes]
+    alone = [Layer(*s, i) for i, s in enumerate(sizes)]
+    for a, t in zip(alone, streams):
+        steps(a, t)
+    both = [Layer(*s, i) for i, s in enumerate(sizes)]
+    threads = [threading.Thread(target=steps, args=x) for x in zip(both, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(alone, both):
+        x, y = a.read(), b.read()
+        assert all(np.array_equal(x[k], y[k]) for k in a.OUT)
